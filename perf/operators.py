@@ -236,7 +236,10 @@ def _call(s):
         w = ea.Int4Weight(dt, c["n"], c["k"], c["group"], s["w"].data_ptr(),
                           s["scales"].data_ptr(), 0 if s["zeros"] is None else s["zeros"].data_ptr())
         y, x, m = s["y"].data_ptr(), s["x"].data_ptr(), c["tokens"]
-        return lambda stream: km.int4_linear(w, m, stream, y, x)
+        need = km.int4_linear_workspace(w, m)
+        s["workspace"] = torch.empty(need, dtype=torch.uint8, device="cuda")
+        ws = (s["workspace"].data_ptr(), need) if need else None
+        return lambda stream: km.int4_linear(w, m, stream, y, x, ws)
     cache = ea.KvCache(dt, c["heads"], c["kv_heads"], c["dim"], s["n_pages"], c["page"],
                        s["k_cache"].data_ptr(), s["v_cache"].data_ptr())
     batch = ea.KvBatch(c["seqs"], s["tokens"], s["offsets"].data_ptr(), s["lens"].data_ptr(),
@@ -250,7 +253,7 @@ def _call(s):
                                            strides)
     need = km.prefix_attention_workspace(cache, c["seqs"], s["tokens"], c["shared"])
     s["workspace"] = torch.empty(need, dtype=torch.uint8, device="cuda")
-    ws = (s["workspace"].data_ptr(), need)
+    ws = (s["workspace"].data_ptr(), need) if need else None
     out, q, shared, scale = s["out"].data_ptr(), s["q"].data_ptr(), c["shared"], s["scale"]
     return lambda stream: km.prefix_attention(cache, batch, shared, scale, stream, out, q, ws)
 
