@@ -14,9 +14,15 @@ from .km import (  # noqa: F401
     F32,
     F64,
     Einsummable,
+    Int4Weight,
     KernelManager,
+    KvBatch,
+    KvCache,
     KmError,
     NodeCallback,
+    ROPE_HALVES,
+    ROPE_NONE,
+    ROPE_PAIRS,
     StreamPool,
     WorkspacePool,
     Touch,

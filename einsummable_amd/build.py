@@ -29,6 +29,10 @@ SOURCES = [
     "gemm_f16.hip",
     "gemm_f32.hip",
     "gemm_f64.hip",
+    "serving.cc",
+    "kv_append.hip",
+    "prefix_attention.hip",
+    "int4_linear.hip",
 ]
 
 COMMON = ["-std=c++17", "-O3", "-fPIC", "-Wall", "-Wno-unused-function"]

@@ -9,6 +9,7 @@
 #include "gemm_kernel.h"
 #include "kernel_manager.h"
 #include "pools.h"
+#include "serving.h"
 #include "static_workspace.h"
 
 #include <cstring>
@@ -103,6 +104,25 @@ int guarded(es_km_t* h, F&& f)
     } catch (std::exception const& e) {
         err_slot(h) = e.what();
         return ES_KM_ERR_DEVICE;
+    }
+}
+
+int unsupported(es_km_t* h, int rc, char const* what)
+{
+    err_slot(h) = std::string(what) + ": no kernel for this dtype or these sizes";
+    return rc;
+}
+
+void check_workspace(void const* workspace, uint64_t bytes, uint64_t needed, char const* what)
+{
+    if (needed == 0) return;
+    if (!workspace || bytes < needed) {
+        throw es::km_error(es::km_status::workspace, std::string(what) + ": needs " +
+                                                         std::to_string(needed) +
+                                                         " bytes of workspace");
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
+        throw es::ir_error(std::string(what) + ": the workspace has to be 256-byte aligned");
     }
 }
 
@@ -353,6 +373,95 @@ int es_km_fill_lowertri(es_km_t* h, int dtype, uint64_t lower_bits, uint64_t upp
         if (!out) throw es::ir_error("fill: null buffer");
         h->km->lowerTri_fill(es::dtype_t(dtype), lower_bits, upper_bits, nrow, ncol, start,
                              static_cast<hipStream_t>(stream), out);
+        return ES_KM_OK;
+    });
+}
+
+int es_km_kv_append(es_km_t* h, const es_km_kv_cache_t* cache, const es_km_kv_batch_t* batch,
+                    void* stream, void* q_out, const void* q, const void* k, const void* v,
+                    uint64_t q_out_stride, uint64_t q_stride, uint64_t k_stride,
+                    uint64_t v_stride, int rope, const void* freqs, uint64_t n_pos)
+{
+    return guarded(h, [&]() -> int {
+        if (!cache || !batch) throw es::ir_error("kv_append: null descriptor");
+        es::kv_append_args_t a{*cache,  *batch,   q,        k,    v, q_out, q_stride, k_stride,
+                               v_stride, q_out_stride, rope, static_cast<const float*>(freqs),
+                               n_pos};
+        if (int const rc = es::check_kv_append(a)) return unsupported(h, rc, "kv_append");
+        if (!h) throw es::ir_error("null handle");
+        es::device_scope_t scope(h->km->device());
+        es::launch_kv_append(a, static_cast<hipStream_t>(stream));
+        return ES_KM_OK;
+    });
+}
+
+int es_km_prefix_attention_workspace(es_km_t* h, const es_km_kv_cache_t* cache, int n_seqs,
+                                     int n_tokens, uint64_t shared, uint64_t* workspace_bytes)
+{
+    return guarded(h, [&]() -> int {
+        if (int const rc = es::check_cache(cache, false)) {
+            return unsupported(h, rc, "prefix_attention");
+        }
+        es_km_kv_batch_t b{};
+        b.n_seqs = n_seqs;
+        b.n_tokens = n_tokens;
+        b.max_pages = 1;
+        b.table_stride = 1;
+        es::check_batch(&b, false);
+        if (shared > (1ull << 30)) {
+            throw es::ir_error("prefix_attention: shared beyond 2^30 positions");
+        }
+        if (!workspace_bytes) throw es::ir_error("prefix_attention: null result");
+        *workspace_bytes = es::plan_attention(*cache, n_seqs, n_tokens, shared).workspace_bytes;
+        return ES_KM_OK;
+    });
+}
+
+int es_km_prefix_attention(es_km_t* h, const es_km_kv_cache_t* cache,
+                           const es_km_kv_batch_t* batch, uint64_t shared, float scale,
+                           void* stream, void* out, const void* q, uint64_t out_stride,
+                           uint64_t q_stride, void* workspace, uint64_t workspace_bytes)
+{
+    return guarded(h, [&]() -> int {
+        if (!cache || !batch) throw es::ir_error("prefix_attention: null descriptor");
+        es::attention_args_t a{*cache, *batch, shared, scale, q, out, q_stride, out_stride};
+        if (int const rc = es::check_attention(a)) return unsupported(h, rc, "prefix_attention");
+        es::attention_plan_t const p =
+            es::plan_attention(*cache, batch->n_seqs, batch->n_tokens, shared);
+        check_workspace(workspace, workspace_bytes, p.workspace_bytes, "prefix_attention");
+        if (!h) throw es::ir_error("null handle");
+        es::device_scope_t scope(h->km->device());
+        es::launch_attention(a, p, workspace, static_cast<hipStream_t>(stream));
+        return ES_KM_OK;
+    });
+}
+
+int es_km_int4_linear_workspace(es_km_t* h, const es_km_int4_weight_t* weight, uint64_t m,
+                                uint64_t* workspace_bytes)
+{
+    return guarded(h, [&]() -> int {
+        if (int const rc = es::check_int4_weight(weight, false)) {
+            return unsupported(h, rc, "int4_linear");
+        }
+        if (m > 65536) throw es::ir_error("int4_linear: more than 65536 tokens");
+        if (!workspace_bytes) throw es::ir_error("int4_linear: null result");
+        *workspace_bytes = es::int4_workspace(*weight, m);
+        return ES_KM_OK;
+    });
+}
+
+int es_km_int4_linear(es_km_t* h, const es_km_int4_weight_t* weight, uint64_t m, void* stream,
+                      void* y, const void* x, uint64_t y_stride, uint64_t x_stride,
+                      void* workspace, uint64_t workspace_bytes)
+{
+    return guarded(h, [&]() -> int {
+        if (!weight) throw es::ir_error("int4 weight: null descriptor");
+        es::int4_args_t a{*weight, m, x, y, x_stride, y_stride};
+        if (int const rc = es::check_int4_linear(a)) return unsupported(h, rc, "int4_linear");
+        check_workspace(workspace, workspace_bytes, es::int4_workspace(*weight, m), "int4_linear");
+        if (!h) throw es::ir_error("null handle");
+        es::device_scope_t scope(h->km->device());
+        es::launch_int4_linear(a, workspace, static_cast<hipStream_t>(stream));
         return ES_KM_OK;
     });
 }

@@ -5,6 +5,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
 F16, F32, F64, C64 = 0, 1, 2, 3
+ROPE_NONE, ROPE_PAIRS, ROPE_HALVES = 0, 1, 2
 DTYPE_SIZE = {F16: 2, F32: 4, F64: 8, C64: 8}
 
 OK, UNSUPPORTED = 0, 1
@@ -23,6 +24,11 @@ EXPORTS = [
     "es_km_touch_batch",
     "es_km_fill_constant",
     "es_km_fill_lowertri",
+    "es_km_kv_append",
+    "es_km_prefix_attention_workspace",
+    "es_km_prefix_attention",
+    "es_km_int4_linear_workspace",
+    "es_km_int4_linear",
     "es_km_codegen_source",
     "es_km_scalarop_roundtrip",
     "es_km_scalarop_simplify",
@@ -188,6 +194,11 @@ def load_library():
                                                      ctypes.c_void_p, ctypes.c_void_p,
                                                      ctypes.c_void_p, ctypes.c_size_t]
     V, I, U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64
+    lib.es_km_kv_append.argtypes = [V, V, V, V, V, V, V, V, U64, U64, U64, U64, I, V, U64]
+    lib.es_km_prefix_attention_workspace.argtypes = [V, V, I, I, U64, V]
+    lib.es_km_prefix_attention.argtypes = [V, V, V, U64, ctypes.c_float, V, V, V, U64, U64, V, U64]
+    lib.es_km_int4_linear_workspace.argtypes = [V, V, U64, V]
+    lib.es_km_int4_linear.argtypes = [V, V, U64, V, V, V, U64, U64, V, U64]
     lib.es_km_graph_create.restype = V
     lib.es_km_graph_create.argtypes = [V]
     lib.es_km_graph_destroy.argtypes = [V]
@@ -336,6 +347,55 @@ class TouchBatch:
         self.dims = (ctypes.c_uint64 * max(len(flat), 1))(*flat)
         self.ranks = (ctypes.c_int * max(self.n, 1))(*[len(t.selection) for t in touches])
         self.castables = b"".join(_castable_char(t.castable) for t in touches) + b"\0"
+
+
+class KvCache(ctypes.Structure):
+    """es_km_kv_cache_t: a paged cache of keys and values at the device addresses k and v.
+    strides: (page, token, head) in elements; None means dense [page, position, head, element]
+    pages.  n_heads counts the query heads that read it."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_uint64),
+                ("page_stride", ctypes.c_uint64), ("token_stride", ctypes.c_uint64),
+                ("head_stride", ctypes.c_uint64), ("dtype", ctypes.c_int32),
+                ("n_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+    def __init__(self, dtype, n_heads, n_kv_heads, head_dim, n_pages, page_size, k, v,
+                 strides=None):
+        if strides is None:
+            strides = (page_size * n_kv_heads * head_dim, n_kv_heads * head_dim, head_dim)
+        super().__init__(k, v, n_pages, *strides, dtype, n_heads, n_kv_heads, head_dim, page_size)
+        self._at = ctypes.addressof(self)
+
+
+class KvBatch(ctypes.Structure):
+    """es_km_kv_batch_t: the batch's new tokens; device addresses of int32 arrays."""
+
+    _fields_ = [("offsets", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_uint64),
+                ("n_seqs", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32)]
+
+    def __init__(self, n_seqs, n_tokens, offsets, lens, page_table, max_pages, table_stride=None):
+        super().__init__(offsets, lens, page_table,
+                         max_pages if table_stride is None else table_stride, n_seqs, n_tokens,
+                         max_pages)
+        self._at = ctypes.addressof(self)
+
+
+class Int4Weight(ctypes.Structure):
+    """es_km_int4_weight_t: n rows of k 4-bit weights with a scale (and a zero point, or 8) per
+    group; device addresses.  Strides default to dense rows."""
+
+    _fields_ = [("w", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+                ("n", ctypes.c_uint64), ("k", ctypes.c_uint64), ("group", ctypes.c_uint64),
+                ("w_stride", ctypes.c_uint64), ("scale_stride", ctypes.c_uint64),
+                ("dtype", ctypes.c_int32)]
+
+    def __init__(self, dtype, n, k, group, w, scales, zeros=0, w_stride=None, scale_stride=None):
+        super().__init__(w, scales, zeros, n, k, group, k // 2 if w_stride is None else w_stride,
+                         -(-k // group) if scale_stride is None else scale_stride, dtype)
+        self._at = ctypes.addressof(self)
 
 
 def codegen_source(e, compile=False):
@@ -489,6 +549,58 @@ class KernelManager:
     def lowerTri_fill(self, dtype, lower_bits, upper_bits, nrow, ncol, start, stream, out):
         rc = self._lib.es_km_fill_lowertri(self._h, dtype, lower_bits, upper_bits, nrow, ncol,
                                            start, stream, out)
+        if rc != OK:
+            self._fail(rc)
+
+    def kv_append(self, cache, batch, stream, q_out, q, k, v, rope=ROPE_PAIRS, freqs=0, n_pos=0,
+                  strides=None):
+        """Rotates the batch's new queries and keys by their positions and writes keys and
+        values into the cache (es_km_kv_append).  q_out and q may both be 0.  strides:
+        (q_out, q, k, v) in elements from token to token; None means dense rows."""
+        if strides is None:
+            h, kv = cache.n_heads * cache.head_dim, cache.n_kv_heads * cache.head_dim
+            strides = (h, h, kv, kv)
+        rc = self._lib.es_km_kv_append(self._h, cache._at, batch._at, stream, q_out, q, k, v,
+                                       *strides, rope, freqs, n_pos)
+        if rc != OK:
+            self._fail(rc)
+
+    def prefix_attention_workspace(self, cache, n_seqs, n_tokens, shared=0):
+        ws = ctypes.c_uint64(0)
+        rc = self._lib.es_km_prefix_attention_workspace(self._h, cache._at, n_seqs, n_tokens,
+                                                        shared, ctypes.addressof(ws))
+        if rc != OK:
+            self._fail(rc)
+        return ws.value
+
+    def prefix_attention(self, cache, batch, shared, scale, stream, out, q, workspace=None,
+                         strides=None):
+        """Attention of the batch's new tokens over the cache, the first `shared` positions of
+        which are the same for every sequence (es_km_prefix_attention).  strides: (out, q) in
+        elements from token to token; None means dense rows."""
+        if strides is None:
+            strides = (cache.n_heads * cache.head_dim,) * 2
+        ws_ptr, ws_size = workspace if workspace else (None, 0)
+        rc = self._lib.es_km_prefix_attention(self._h, cache._at, batch._at, shared, scale, stream,
+                                              out, q, *strides, ws_ptr, ws_size)
+        if rc != OK:
+            self._fail(rc)
+
+    def int4_linear_workspace(self, weight, m):
+        ws = ctypes.c_uint64(0)
+        rc = self._lib.es_km_int4_linear_workspace(self._h, weight._at, m, ctypes.addressof(ws))
+        if rc != OK:
+            self._fail(rc)
+        return ws.value
+
+    def int4_linear(self, weight, m, stream, y, x, workspace=None, strides=None):
+        """y = x W^T for m tokens (es_km_int4_linear).  strides: (y, x) in elements from token to
+        token; None means dense rows."""
+        if strides is None:
+            strides = (weight.n, weight.k)
+        ws_ptr, ws_size = workspace if workspace else (None, 0)
+        rc = self._lib.es_km_int4_linear(self._h, weight._at, m, stream, y, x, *strides, ws_ptr,
+                                         ws_size)
         if rc != OK:
             self._fail(rc)
 

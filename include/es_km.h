@@ -176,6 +176,127 @@ double es_km_probe_mfma_f16(es_km_t* km, const void* operands, void* scratch, in
                             void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Serving operators: what a decoder layer needs to run token by token, on a paged cache of
+ * keys and values.  No counterpart in the reference, whose LLaMA recomputes the whole prompt
+ * (attention_t::forward, llama/modules.cc:282-356) or concatenates the cache as a tensor.
+ * They stand beside es_km_touch: no build, raw device pointers, everything asynchronous on
+ * `stream`, nothing allocated, no state kept between calls, so calls may be captured into HIP
+ * graphs.  dtype is ES_KM_F16 or ES_KM_F32 (arithmetic in fp32 either way); for the other two
+ * ES_KM_UNSUPPORTED comes back.  Arguments are checked before anything is launched; `km` NULL
+ * gets the checks and then ES_KM_ERR_INVALID.
+ *
+ * The cache: n_pages pages of page_size positions, an entry (head_dim elements, contiguous)
+ * per position and key head at  base + page * page_stride + row * token_stride + head *
+ * head_stride  elements, for keys and values alike.  Strides and bases sit on 16-byte
+ * boundaries; head_dim is a multiple of 8, at most 256; n_heads (query heads) is a multiple
+ * of n_kv_heads, and query head h reads key head h / (n_heads / n_kv_heads).  Dense
+ * [page, position, head, element] pages have the strides (page_size * n_kv_heads * head_dim,
+ * n_kv_heads * head_dim, head_dim), dense [page, head, position, element] ones
+ * (n_kv_heads * page_size * head_dim, head_dim, page_size * head_dim).
+ *
+ * The batch: n_seqs sequences whose new tokens lie behind each other: sequence s owns tokens
+ * offsets[s] .. offsets[s+1]-1 (none is fine) of n_tokens rows.  lens[s] counts all positions
+ * of the sequence, its new tokens included, so token i sits at position
+ * lens[s] - (offsets[s+1] - i).  page_table[s * table_stride + p / page_size] is the page of
+ * its position p, max_pages columns.  The three arrays are int32 on the device and are read
+ * by the kernels, so a captured graph sees their values at replay.  Tokens from
+ * offsets[n_seqs] on (a padded batch) belong to nobody: their rows of every output stay as
+ * they were.  A page number outside 0 .. n_pages-1 means that there is no such page. */
+typedef struct es_km_kv_cache {
+    void*    k;             /* device, like v */
+    void*    v;
+    uint64_t n_pages;
+    uint64_t page_stride;   /* elements */
+    uint64_t token_stride;
+    uint64_t head_stride;
+    int32_t  dtype;
+    int32_t  n_heads;
+    int32_t  n_kv_heads;
+    int32_t  head_dim;
+    int32_t  page_size;
+} es_km_kv_cache_t;
+
+typedef struct es_km_kv_batch {
+    const int32_t* offsets;     /* n_seqs + 1, ascending, on the device like the next two */
+    const int32_t* lens;        /* n_seqs */
+    const int32_t* page_table;  /* n_seqs rows of max_pages */
+    uint64_t       table_stride;
+    int32_t        n_seqs;
+    int32_t        n_tokens;
+    int32_t        max_pages;
+} es_km_kv_batch_t;
+
+/* Appends the new tokens' keys and values to the cache and rotates queries and keys by their
+ * positions on the way (the rotary embedding of llama/modules.cc:257-279, there a product of
+ * c64 views).  q, k, v: rows of n_heads, n_kv_heads, n_kv_heads heads, *_stride elements from
+ * token to token (a packed projection's output is three pointers into it).  q_out may be q
+ * itself, or q and q_out both NULL: keys and values only.
+ *   rope ES_KM_ROPE_NONE    no rotation, freqs NULL
+ *   rope ES_KM_ROPE_PAIRS   elements (2j, 2j+1) are a complex number, multiplied by
+ *                           freqs[position][j] -- what the c64 view computes
+ *   rope ES_KM_ROPE_HALVES  elements (j, j + head_dim/2) are
+ * freqs: n_pos rows of head_dim/2 c64 (full_freqs_cis, llama/modules.cc:578-605), f32 pairs
+ * on an 8-byte boundary.  Products and sums in fp32, rounded once.  Nothing is written of a
+ * token whose position is negative or has no row of freqs; keys and values of a position
+ * without a page are dropped, its q_out is written. */
+enum { ES_KM_ROPE_NONE = 0, ES_KM_ROPE_PAIRS = 1, ES_KM_ROPE_HALVES = 2 };
+int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_batch_t* batch,
+                    void* stream, void* q_out, const void* q, const void* k, const void* v,
+                    uint64_t q_out_stride, uint64_t q_stride, uint64_t k_stride,
+                    uint64_t v_stride, int rope, const void* freqs, uint64_t n_pos);
+
+/* Attention of the new tokens over the cache, theirs included:
+ *   out[i, h] = sum_j p_j V[j, h'],  p = softmax_j(scale * q[i, h] . K[j, h'])
+ * over the positions j of token i's sequence up to its own (h' the key head of h).  The first
+ * `shared` positions hold the same keys and values for every sequence of the batch (a common
+ * prefix): they are read through the page table's first row, once for the rows of many
+ * sequences together; 0 when nothing is shared.  The result is the same for every `shared`
+ * that is true of the batch.  A sequence may be shorter than `shared`.
+ * Positions whose page does not exist, or beyond max_pages, are left out; a token without any
+ * position gets zeros.  What masked positions hold, infinities and NaN included, has no
+ * influence; neither have cache entries beyond lens.
+ * q and out: n_heads heads per token, q_stride / out_stride elements from token to token, on
+ * 16-byte boundaries; out may not overlap q or the cache.
+ * workspace: es_km_prefix_attention_workspace bytes on a 256-byte boundary, used from the
+ * call until its work is done (calls that overlap in time need one each), contents irrelevant
+ * before and after. */
+int es_km_prefix_attention_workspace(es_km_t* km, const es_km_kv_cache_t* cache, int n_seqs,
+                                     int n_tokens, uint64_t shared, uint64_t* workspace_bytes);
+int es_km_prefix_attention(es_km_t* km, const es_km_kv_cache_t* cache,
+                           const es_km_kv_batch_t* batch, uint64_t shared, float scale,
+                           void* stream, void* out, const void* q, uint64_t out_stride,
+                           uint64_t q_stride, void* workspace, uint64_t workspace_bytes);
+
+/* Products with a 4-bit weight, y[i, n] = sum_k x[i, k] W[n, k] (the node "ij,kj->ik" of a
+ * linear layer) with
+ *   W[n, k] = scales[n, k / group] * (nibble(n, k) - zeros[n, k / group])
+ * nibble(n, k): bits 4 (k % 2) .. of byte k / 2 of row n (the lower nibble is the even k),
+ * w_stride bytes from row to row; scales: the dtype of x and y; zeros: uint8, or NULL for 8
+ * everywhere; both ceil(k / group) to a row, rows scale_stride apart.  k and group are
+ * multiples of 32, group at least 32; x and w (bases and strides) sit on 16-byte boundaries.
+ * Meant for few tokens (m): the weight is streamed once per 64 of them (f16; 16 in f32).
+ * Products of integers and activations are exact, sums fp32.  f32 activations are split into
+ * three f16 parts relative to their row's largest magnitude (33 bits in all) in the
+ * workspace, whose size es_km_int4_linear_workspace reports (0 for f16). */
+typedef struct es_km_int4_weight {
+    const void*    w;       /* device, like the next two */
+    const void*    scales;
+    const uint8_t* zeros;
+    uint64_t       n;
+    uint64_t       k;
+    uint64_t       group;
+    uint64_t       w_stride;      /* bytes */
+    uint64_t       scale_stride;  /* elements, of scales and of zeros */
+    int32_t        dtype;
+} es_km_int4_weight_t;
+
+int es_km_int4_linear_workspace(es_km_t* km, const es_km_int4_weight_t* weight, uint64_t m,
+                                uint64_t* workspace_bytes);
+int es_km_int4_linear(es_km_t* km, const es_km_int4_weight_t* weight, uint64_t m, void* stream,
+                      void* y, const void* x, uint64_t y_stride, uint64_t x_stride,
+                      void* workspace, uint64_t workspace_bytes);
+
+/* ---------------------------------------------------------------------------------------
  * Exec-node layer: a dependency graph of apply / fill / copy nodes over ONE device arena.
  *
  * Replaces, for one GPU, the reference's GPU exec graph and its node types
