@@ -17,15 +17,19 @@
 // has no preferred order).  Neither K nor V nor P passes through LDS.  A lane's rows of V are
 // consecutive elements of 4 or 8 keys; in f16 they are transposed in registers (v_perm_b32).
 //
-// A workgroup is four wavefronts that take the steps of its keys in turn and join their m, l
-// and O at the end through LDS.  Work is cut over the keys: "prefix" workgroups take the rows
-// of the whole batch against a cut of the shared positions, the others the rows of one sequence
-// against a cut of its own positions.  How many cuts a sequence gets follows from the lengths
-// in device memory (every workgroup adds them up for itself: the host knows only the number of
-// sequences and tokens, and a captured graph must see the lengths of the day).  Each cut leaves
-// O, m, l in fp32 in the workspace; attention_join_kernel adds them in a fixed order, so
-// results do not depend on timing.  A row whose keys were all in one workgroup is stored
-// directly.
+// Two kernels.  attention_few_kernel, for decoding: tiles of 16 rows; the four wavefronts of a
+// workgroup take the steps of its keys in turn, straight from global memory into registers (K
+// and V are used once), and join their m, l and O at the end through LDS.  attention_many_kernel,
+// for the shared positions of a batch and for prompts: each wavefront has 16 or 32 rows of its
+// own and all of them go through the same tiles of keys, staged in LDS.
+//
+// Work is cut over the keys: "prefix" workgroups take the rows of the whole batch against a cut
+// of the shared positions, the others the rows of one sequence against a cut of its own
+// positions.  How many cuts a sequence gets follows from the lengths in device memory (every
+// workgroup adds them up for itself: the host knows only the number of sequences and tokens, and
+// a captured graph must see the lengths of the day).  Each cut leaves O, m, l in fp32 in the
+// workspace; attention_join_kernel adds them in a fixed order, so results do not depend on
+// timing.  A row whose keys were all in one workgroup is stored directly.
 #include "kernel_manager.h"
 #include "serving.h"
 #include "serving_device.h"
@@ -38,7 +42,6 @@ namespace es
 namespace
 {
 
-constexpr int ROWS = 16;     // queries per tile
 constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / 64;
 
@@ -55,12 +58,16 @@ struct attention_dev_t {
     int         h_kv, group, d;
     int         shared;
     float       scale;  // of the scores, times log2(e)
-    int         prefix_tiles, prefix_splits, prefix_chunk;
+    uint32_t    page_magic, page_shift;
+    int         prefix_tiles, prefix_splits, prefix_chunk, prefix_rows;
     int         split_target;
-    int         items;
-    float*      part_o;     // [slot][key head][16][D]
-    float*      part_ml;    // [slot][key head][16][2]
-    int*        part_meta;  // [token][4]: slot of its tile's first cut, cuts, first token, -
+    int         items, own_rows;
+    int         parts;      // what this launch does: 1 prefix, 2 own positions, 3 both
+    int         direct;     // there are no shared positions to join with
+    float*      part_o;     // [row of a slot][D]: the prefix's slots, then the own ones
+    float*      part_ml;    // [row of a slot][2]
+    int*        part_meta;  // [token][4]: first cut of the sequence's first tile, cuts, token 0
+    int64_t     own_base;   // rows before the own positions' slots
 };
 
 constexpr float NEG_INF = -__builtin_huge_valf();
@@ -74,13 +81,193 @@ __device__ inline long long wave_sum(long long v)
     return v;
 }
 
-// The lane that owns a row's column also knows where the row ends up.
-struct rows_t {
-    int  token = -1;  // of this lane's column (-1: no such row)
-    int  head = 0;
-    int  limit = 0x7fffffff;  // its last position
-    int  least = 0x7fffffff;  // the least limit of the tile's rows
+// pos / page_size, exact below 2^30 positions
+__device__ inline int page_of(attention_dev_t const& a, int pos)
+{
+    return int((uint64_t(uint32_t(pos)) * a.page_magic) >> a.page_shift);
+}
+
+// Element offset of a position's entry for key head 0; -1: no such page.
+__device__ inline int64_t entry_of(attention_dev_t const& a, int page, int row)
+{
+    if (page < 0 || uint64_t(page) >= a.n_pages) return -1;
+    return int64_t(uint64_t(page) * a.page_stride + uint64_t(row) * a.token_stride);
+}
+
+// What a workgroup was given: the positions lo <= p < hi of a page table's row, and a tile of
+// rows, which are either rows of the whole batch or of one sequence.
+struct work_t {
+    int        lo, hi;
+    int const* table;
+    int64_t    part;    // first row of its slot
+    bool       direct;
+    bool       whole;   // rows of the whole batch, positions in limit[]
+    int        r0;      // first row, counted from token b
+    int        b, e;    // tokens
+    int        end, len;  // of the sequence: its last token + 1, positions
 };
+
+// The row that a lane deals with.
+struct row_t {
+    int token = -1;  // -1: no such row
+    int head = 0;
+    int limit = 0x7fffffff;  // its last position
+};
+
+struct deal_t {
+    long long total[WAVES];
+    int       before[WAVES];
+    int       found[4];  // sequence, item within it, first slot, cuts
+};
+
+template <int ROWS>
+__device__ inline row_t row_of(attention_dev_t const& a, work_t const& k, int const* limit, int kvh,
+                               int i)
+{
+    row_t     row;
+    int const r = k.r0 + i;
+    int const j = r / a.group;
+    int const t = k.b + j;
+    if (t >= k.e) return row;
+    int at;
+    if (k.whole) {
+        at = limit[j - k.r0 / a.group];
+        if (at == -2) return row;
+    } else {
+        at = max(k.len - (k.end - t), -1);
+    }
+    row.token = t;
+    row.head = kvh * a.group + r - j * a.group;
+    row.limit = at;
+    return row;
+}
+
+// Finds the workgroup's work; false: there is none.  `limit` holds ROWS ints.
+template <int ROWS, int KS>
+__device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit, int kvh, work_t& k)
+{
+    int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
+    int const prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
+    int const reach = a.max_pages * a.page_size;  // positions that a table row has pages for
+    if (unit < prefix_units) {
+        int const tile = unit % a.prefix_tiles;
+        int const split = unit / a.prefix_tiles;
+        k.part = (int64_t(unit) * a.h_kv + kvh) * ROWS;
+        k.lo = split * a.prefix_chunk;
+        k.hi = min(min(k.lo + a.prefix_chunk, a.shared), reach);
+        k.table = a.table;
+        k.direct = false;
+        k.whole = true;
+        k.r0 = tile * ROWS;
+        k.b = 0;
+        int const t0 = k.r0 / a.group;
+        k.e = min((k.r0 + ROWS - 1) / a.group + 1, a.n_tokens);
+        k.end = k.len = 0;
+        for (int i = tid; i < ROWS; i += THREADS) limit[i] = -2;
+        __syncthreads();
+        // each thread puts down the positions of the tile's tokens in its sequences
+        for (int s = tid; s < a.n_seqs; s += THREADS) {
+            int const b = a.offsets[s], e = a.offsets[s + 1];
+            int const len = a.lens[s];
+            for (int t = max(b, t0); t < min(e, k.e); ++t) {
+                limit[t - t0] = max(len - (e - t), -1);
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+    // The cuts of all sequences, numbered through: tiles_s * splits_s each, where a cut holds
+    // `chunk` steps.  A thread adds up a run of sequences.
+    int const item = unit - prefix_units;
+    int const run = (a.n_seqs + THREADS - 1) / THREADS;
+    int const s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
+    if (tid == 0) sh.found[0] = -1;
+    long long total = 0;
+    auto tiles_steps = [&](int s, int& tiles, int& steps) {
+        int const b = max(a.offsets[s], 0), e = min(a.offsets[s + 1], a.n_tokens);
+        int const len = min(a.lens[s], reach);
+        tiles = e > b ? ((e - b) * a.group + ROWS - 1) / ROWS : 0;
+        steps = len > a.shared ? (len + KS - 1) / KS - a.shared / KS : 0;
+    };
+    int tiles = 0, steps = 0;
+    for (int s = s0; s < s1; ++s) {
+        tiles_steps(s, tiles, steps);
+        total += (long long)tiles * steps;
+    }
+    long long const ws = wave_sum(total);
+    if (lane == 0) sh.total[w] = ws;
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int i = 0; i != WAVES; ++i) all += sh.total[i];
+    // a multiple of four steps: one for each wavefront that takes them in turn
+    int chunk = 0x3fffffff;
+    if (a.split_target > 0) {
+        long long const per = (all + a.split_target - 1) / a.split_target;
+        chunk = int(max((long long)WAVES, (per + WAVES - 1) / WAVES * WAVES));
+    }
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        if (run > 1) tiles_steps(s, tiles, steps);
+        mine += tiles * max(1, (steps + chunk - 1) / chunk);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        int const up = __shfl_up(incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 63) sh.before[w] = incl;
+    __syncthreads();
+    int start = incl - mine;
+#pragma unroll
+    for (int i = 0; i != WAVES; ++i) start += i < w ? sh.before[i] : 0;
+    if (item >= start && item < start + mine) {
+        for (int s = s0; s < s1; ++s) {
+            if (run > 1) tiles_steps(s, tiles, steps);
+            int const splits = max(1, (steps + chunk - 1) / chunk);
+            if (item < start + tiles * splits) {
+                sh.found[0] = s;
+                sh.found[1] = item - start;
+                sh.found[2] = start;
+                sh.found[3] = splits;
+                break;
+            }
+            start += tiles * splits;
+        }
+    }
+    __syncthreads();
+    int const s = sh.found[0];
+    if (s < 0) return false;
+    int const splits = sh.found[3];
+    int const tile = sh.found[1] / splits, split = sh.found[1] - tile * splits;
+    k.b = max(a.offsets[s], 0);
+    k.e = min(a.offsets[s + 1], a.n_tokens);
+    k.end = a.offsets[s + 1];
+    k.len = a.lens[s];
+    k.whole = false;
+    k.part = a.own_base + (int64_t(item) * a.h_kv + kvh) * ROWS;
+    k.direct = splits == 1 && a.direct;
+    k.table = a.table + uint64_t(s) * a.table_stride;
+    k.r0 = tile * ROWS;
+    int const last = min(k.e - 1, k.b + (k.r0 + ROWS - 1) / a.group);
+    if (split == 0 && kvh == 0) {
+        int const first = k.b + k.r0 / a.group;
+        for (int t = first + tid; t <= last; t += THREADS) {
+            int* const meta = a.part_meta + 4 * t;
+            meta[0] = sh.found[2];
+            meta[1] = k.direct ? 0 : splits;
+            meta[2] = k.b;
+        }
+    }
+    // positions of this cut, up to the last one that a row of the tile sees
+    int const len = min(k.len, reach);
+    int const step0 = a.shared / KS + (splits == 1 ? 0 : split * chunk);
+    k.lo = max(a.shared, step0 * KS);
+    k.hi = splits == 1 ? len : min(len, (step0 + chunk) * KS);
+    k.hi = min(k.hi, k.len - (k.end - last) + 1);
+    return true;
+}
 
 template <typename T, int D>
 struct core_t;
@@ -294,27 +481,29 @@ struct core_t<float, D> {
     }
 };
 
+// ------------------------------------------------------------------------------ few rows
+
+constexpr int FEW = 16;
+
 template <typename T, int D>
-struct shared_t {
+struct few_shared_t {
     static constexpr int DJ = D < 128 ? D : 128;  // elements joined at a time
+    deal_t  deal;
+    int     limit[FEW];
     int64_t off[WAVES][32];
-    float   m[WAVES][ROWS], l[WAVES][ROWS];
-    float   o[WAVES][ROWS][DJ + 4];
-    long long total[WAVES];
-    int     before[WAVES];
-    int     found[4];  // sequence, item within it, first slot, cuts
-    int     limit[ROWS];
+    float   m[WAVES][FEW], l[WAVES][FEW];
+    float   o[WAVES][FEW][DJ + 4];
 };
 
-// The keys lo <= position < hi of one table row against the tile's rows; steps w, w + WAVES, ...
+// The workgroup's keys against the tile's rows; steps w, w + WAVES, ...
 template <typename T, int D>
-__device__ void attend(attention_dev_t const& a, shared_t<T, D>& sh, rows_t const& row,
-                       int const* __restrict__ table, int kvh, int lo, int hi, float4_t* o,
-                       float& m, float& l)
+__device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const& wk, row_t const& row,
+                           int least, int kvh, float4_t* o, float& m, float& l)
 {
     typedef core_t<T, D> core;
     constexpr int        KS = core::KS, KL = core::KL, DV = core::DV;
-    int const            lane = int(threadIdx.x) & 63, w = int(threadIdx.x) >> 6;
+    int const            lane = int(threadIdx.x) & 63;
+    int const            w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     int const            g = lane >> 4, c = lane & 15;
     T const* const       kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
     T const* const       vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
@@ -323,28 +512,34 @@ __device__ void attend(attention_dev_t const& a, shared_t<T, D>& sh, rows_t cons
                            : reinterpret_cast<T const*>(a.q) + uint64_t(row.token) * a.q_stride +
                                  uint64_t(row.head) * uint64_t(a.d),
              g, a.d);
-    int64_t* const off = sh.off[w];
-    for (int base = (lo / KS + w) * KS; base < hi; base += WAVES * KS) {
-        // where the step's keys lie; -1: not among them, or no such page
-        int     pos = base + (lane & (KS - 1));
-        int64_t at = -1;
+    int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
+    int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
+    int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
+    // a step ahead: the page of this lane's key (-1: not among them, or no such page)
+    int  page = -1, prow = 0;
+    auto look_up = [&](int base) {
+        int const pos = base + (lane & (KS - 1));
+        page = -1;
         if (pos >= lo && pos < hi) {
-            int const pi = pos / a.page_size;
-            int const page = table[pi];
-            if (page >= 0 && uint64_t(page) < a.n_pages) {
-                at = int64_t(uint64_t(page) * a.page_stride +
-                             uint64_t(pos - pi * a.page_size) * a.token_stride);
-            }
+            int const pi = page_of(a, pos);
+            prow = pos - pi * a.page_size;
+            page = wk.table[pi];
         }
-        bool const holes = __any(at < 0);
+    };
+    int base = (lo / KS + w) * KS;
+    look_up(base);
+    for (; base < hi; base += WAVES * KS) {
+        int64_t const at = entry_of(a, page, prow);
+        bool const    holes = __any(at < 0);
         __builtin_amdgcn_wave_barrier();
         if (lane < KS) off[lane] = at;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        look_up(base + WAVES * KS);
         x.load(kb, vb, off, c, g, a.d);
         float s[KL];
         x.scores(s);
-        bool const edge = holes || base + KS - 1 > row.least;
+        bool const edge = holes || base + KS - 1 > seen_by_all;
         uint32_t   masked = 0;
         if (edge) {
 #pragma unroll
@@ -389,7 +584,7 @@ __device__ void attend(attention_dev_t const& a, shared_t<T, D>& sh, rows_t cons
         if (!careful) {
             x.template values<false>(s, o, 0, true);
         } else {
-            for (int r = 0; r != ROWS; ++r) {
+            for (int r = 0; r != FEW; ++r) {
                 int const limit = __shfl(row.limit, r);
                 uint32_t  seen = 0;
 #pragma unroll
@@ -406,157 +601,27 @@ __device__ void attend(attention_dev_t const& a, shared_t<T, D>& sh, rows_t cons
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(THREADS) void attention_kernel(attention_dev_t a)
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kernel(attention_dev_t a)
 {
-    __shared__ shared_t<T, D> sh;
+    __shared__ few_shared_t<T, D> sh;
     int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
     int const c = lane & 15, g = lane >> 4;
     int const kvh = int(blockIdx.x) % a.h_kv;
-    int const unit = int(blockIdx.x) / a.h_kv;
-    int const prefix_units = a.prefix_tiles * a.prefix_splits;
-    int const reach = a.max_pages * a.page_size;  // positions that a table row has pages for
-
-    rows_t     row;
-    int        lo, hi, slot;
-    int const* table = a.table;
-    bool       direct = false;
-    if (unit < prefix_units) {
-        int const tile = unit % a.prefix_tiles;
-        int const split = unit / a.prefix_tiles;
-        slot = unit;
-        lo = split * a.prefix_chunk;
-        hi = min(min(lo + a.prefix_chunk, a.shared), reach);
-        int const r0 = tile * ROWS;
-        int const t0 = r0 / a.group;
-        int const t1 = min((r0 + ROWS - 1) / a.group, a.n_tokens - 1);
-        if (tid < ROWS) sh.limit[tid] = -2;
-        __syncthreads();
-        // each thread puts down the positions of the tile's tokens in its sequences
-        for (int s = tid; s < a.n_seqs; s += THREADS) {
-            int const b = a.offsets[s], e = a.offsets[s + 1];
-            if (b > t1 || e <= t0) continue;
-            int const len = a.lens[s];
-            for (int t = max(b, t0); t <= min(e - 1, t1); ++t) {
-                sh.limit[t - t0] = max(len - (e - t), -1);
-            }
-        }
-        __syncthreads();
-        int const r = r0 + c;
-        int const t = r / a.group;
-        if (t <= t1 && sh.limit[t - t0] != -2) {
-            row.token = t;
-            row.head = kvh * a.group + r - t * a.group;
-            row.limit = sh.limit[t - t0];
-        }
-    } else {
-        // The cuts of all sequences, numbered through: tiles_s * splits_s each, where a cut holds
-        // `chunk` steps.  A thread adds up a run of sequences.
-        constexpr int KS = core_t<T, D>::KS;
-        int const     item = unit - prefix_units;
-        int const     run = (a.n_seqs + THREADS - 1) / THREADS;
-        int const     s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
-        if (tid == 0) sh.found[0] = -1;
-        long long total = 0;
-        auto tiles_steps = [&](int s, int& tiles, int& steps) {
-            int const b = max(a.offsets[s], 0), e = min(a.offsets[s + 1], a.n_tokens);
-            int const len = min(a.lens[s], reach);
-            tiles = e > b ? ((e - b) * a.group + ROWS - 1) / ROWS : 0;
-            steps = len > a.shared ? (len + KS - 1) / KS - a.shared / KS : 0;
-        };
-        int tiles = 0, steps = 0;
-        for (int s = s0; s < s1; ++s) {
-            tiles_steps(s, tiles, steps);
-            total += (long long)tiles * steps;
-        }
-        long long const ws = wave_sum(total);
-        if (lane == 0) sh.total[w] = ws;
-        __syncthreads();
-        long long all = 0;
-#pragma unroll
-        for (int i = 0; i != WAVES; ++i) all += sh.total[i];
-        // at least one step per wavefront
-        int chunk = 0x3fffffff;
-        if (a.split_target > 0) {
-            long long const per = (all + a.split_target - 1) / a.split_target;
-            chunk = int(max((long long)WAVES, (per + WAVES - 1) / WAVES * WAVES));
-        }
-        int mine = 0;
-        for (int s = s0; s < s1; ++s) {
-            if (run > 1) tiles_steps(s, tiles, steps);
-            mine += tiles * max(1, (steps + chunk - 1) / chunk);
-        }
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            int const up = __shfl_up(incl, o);
-            if (lane >= o) incl += up;
-        }
-        if (lane == 63) sh.before[w] = incl;
-        __syncthreads();
-        int start = incl - mine;
-#pragma unroll
-        for (int i = 0; i != WAVES; ++i) start += i < w ? sh.before[i] : 0;
-        if (item >= start && item < start + mine) {
-            for (int s = s0; s < s1; ++s) {
-                if (run > 1) tiles_steps(s, tiles, steps);
-                int const splits = max(1, (steps + chunk - 1) / chunk);
-                if (item < start + tiles * splits) {
-                    sh.found[0] = s;
-                    sh.found[1] = item - start;
-                    sh.found[2] = start;
-                    sh.found[3] = splits;
-                    break;
-                }
-                start += tiles * splits;
-            }
-        }
-        __syncthreads();
-        int const s = sh.found[0];
-        if (s < 0) return;
-        int const splits = sh.found[3];
-        int const tile = sh.found[1] / splits, split = sh.found[1] - tile * splits;
-        int const b = max(a.offsets[s], 0), e = min(a.offsets[s + 1], a.n_tokens);
-        int const true_end = a.offsets[s + 1];
-        int const full = a.lens[s];
-        int const len = min(full, reach);
-        slot = prefix_units + item;
-        direct = splits == 1 && prefix_units == 0;
-        table = a.table + uint64_t(s) * a.table_stride;
-        int const r0 = tile * ROWS;
-        int const r = r0 + c;
-        int const t = b + r / a.group;
-        if (t < e) {
-            row.token = t;
-            row.head = kvh * a.group + r % a.group;
-            row.limit = max(full - (true_end - t), -1);
-        }
-        int const last = min(e - 1, b + (r0 + ROWS - 1) / a.group);
-        if (split == 0 && kvh == 0) {
-            int const first = b + r0 / a.group;
-            if (first + tid <= last) {
-                int* const meta = a.part_meta + 4 * (first + tid);
-                meta[0] = slot - tile * splits;  // of the sequence's first tile
-                meta[1] = direct ? 0 : splits;
-                meta[2] = b;
-            }
-        }
-        // positions of this cut, up to the last one that a row of the tile sees
-        int const step0 = a.shared / KS + (splits == 1 ? 0 : split * chunk);
-        lo = max(a.shared, step0 * KS);
-        hi = splits == 1 ? len : min(len, (step0 + chunk) * KS);
-        hi = min(hi, full - (true_end - last) + 1);
+    work_t    wk;
+    if (!deal<FEW, core_t<T, D>::KS>(a, sh.deal, sh.limit, int(blockIdx.x) / a.h_kv, kvh, wk)) {
+        return;
     }
-    int least = row.limit;
+    row_t const row = row_of<FEW>(a, wk, sh.limit, kvh, c);
+    int         least = row.limit;
 #pragma unroll
     for (int i = 1; i != 16; i <<= 1) least = min(least, __shfl_xor(least, i));
-    row.least = least;
 
     constexpr int DV = core_t<T, D>::DV;
     float4_t      o[DV];
 #pragma unroll
     for (int t = 0; t != DV; ++t) o[t] = float4_t{0, 0, 0, 0};
     float m = NEG_INF, l = 0;
-    if (lo < hi) attend<T, D>(a, sh, row, table, kvh, lo, hi, o, m, l);
+    if (wk.lo < wk.hi) attend_few<T, D>(a, sh.off[w], wk, row, least, kvh, o, m, l);
 
     // join the wavefronts
     if (g == 0) {
@@ -567,10 +632,9 @@ __global__ __launch_bounds__(THREADS) void attention_kernel(attention_dev_t a)
     float top = NEG_INF;
 #pragma unroll
     for (int i = 0; i != WAVES; ++i) top = fmaxf(top, sh.m[i][c]);
-    float const mine = exp2_fast(m - (top == NEG_INF ? 0.0f : top));
-    float*      part = a.part_o + (uint64_t(slot) * uint64_t(a.h_kv) + uint64_t(kvh)) * ROWS * D;
-    constexpr int DJ = shared_t<T, D>::DJ;
-    constexpr int TPR = THREADS / ROWS;  // threads that store a row
+    float const   mine = exp2_fast(m - (top == NEG_INF ? 0.0f : top));
+    constexpr int DJ = few_shared_t<T, D>::DJ;
+    constexpr int TPR = THREADS / FEW;  // threads that store a row
     constexpr int PER = DJ / TPR;
     int const     orow = tid / TPR, oe = tid % TPR * PER;
     // the row that this thread stores, from the lane that knows it
@@ -603,7 +667,7 @@ __global__ __launch_bounds__(THREADS) void attention_kernel(attention_dev_t a)
 #pragma unroll
                 for (int i = 0; i != WAVES; ++i) y[e] += sh.o[i][orow][oe + e];
             }
-            if (direct) {
+            if (wk.direct) {
                 T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(otoken) * a.out_stride +
                                uint64_t(ohead) * uint64_t(a.d) + h * DJ + oe;
                 float const inv = otop == NEG_INF ? 0.0f : 1.0f / sum;
@@ -612,7 +676,7 @@ __global__ __launch_bounds__(THREADS) void attention_kernel(attention_dev_t a)
                     if (h * DJ + oe + e < a.d) dst[e] = T(otop == NEG_INF ? 0.0f : y[e] * inv);
                 }
             } else {
-                float* const dst = part + orow * D + h * DJ + oe;
+                float* const dst = a.part_o + (wk.part + orow) * D + h * DJ + oe;
 #pragma unroll
                 for (int e = 0; e != PER; e += 4) {
                     *reinterpret_cast<float4_t*>(dst + e) =
@@ -621,11 +685,319 @@ __global__ __launch_bounds__(THREADS) void attention_kernel(attention_dev_t a)
             }
         }
     }
-    if (!direct && otoken >= 0 && oe == 0) {
-        float* const ml = a.part_ml +
-                          ((uint64_t(slot) * uint64_t(a.h_kv) + uint64_t(kvh)) * ROWS + orow) * 2;
-        ml[0] = otop;
-        ml[1] = sum;
+    if (!wk.direct && otoken >= 0 && oe == 0) {
+        a.part_ml[(wk.part + orow) * 2] = otop;
+        a.part_ml[(wk.part + orow) * 2 + 1] = sum;
+    }
+}
+
+// ------------------------------------------------------------------------------ many rows
+
+// f16 only.  A tile of KT keys lies in LDS as rows of D elements, 16-byte chunks XOR-swizzled with
+// the row: K by row % 16 (a fragment read takes one chunk of 16 rows), V by 2 (row % 8) (a
+// transposing read takes 32 bytes of four rows).  Two tiles alternate: while one is worked on the
+// next is on its way from global memory to registers, to be put down before the barrier.
+template <int D, int NT>
+struct many_t {
+    static constexpr int ROWS = WAVES * 16 * NT;
+    static constexpr int KT = D == 256 ? 32 : 64;
+    static constexpr int CH = D / 8;                   // chunks per row
+    static constexpr int PASS = KT * CH / THREADS;     // chunks per thread, of K and of V each
+    static constexpr int RPP = THREADS / CH;           // rows per pass
+    static constexpr int DT = D / 16;
+    struct shared_t {
+        deal_t   deal;
+        int      limit[ROWS];
+        int64_t  off[2][KT];
+        int      bad[3];  // of a tile modulo 3: reset a barrier before it is set again
+        half8_t  k[2][KT][CH], v[2][KT][CH];
+    };
+};
+
+template <int D, int NT>
+__global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_dev_t a)
+{
+    typedef many_t<D, NT> M;
+    typedef _Float16      T;
+    constexpr int         ROWS = M::ROWS, KT = M::KT, CH = M::CH, PASS = M::PASS, DT = M::DT;
+    __shared__ typename M::shared_t sh;
+    int const tid = int(threadIdx.x), lane = tid & 63;
+    int const w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int const c = lane & 15, g = lane >> 4;
+    int const kvh = int(blockIdx.x) % a.h_kv;
+    work_t    wk;
+    if (!deal<ROWS, 32>(a, sh.deal, sh.limit, int(blockIdx.x) / a.h_kv, kvh, wk)) return;
+    row_t row[NT];
+    int   least = 0x7fffffff, most = -1;
+#pragma unroll
+    for (int n = 0; n != NT; ++n) {
+        row[n] = row_of<ROWS>(a, wk, sh.limit, kvh, (w * NT + n) * 16 + c);
+        least = min(least, row[n].limit);
+        if (row[n].token >= 0) most = max(most, row[n].limit);
+    }
+#pragma unroll
+    for (int i = 1; i != 16; i <<= 1) {
+        least = min(least, __shfl_xor(least, i));
+        most = max(most, __shfl_xor(most, i));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
+    int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
+
+    half8_t  q[NT][D / 32];
+    float4_t o[NT][DT];
+    float    m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n != NT; ++n) {
+        T const* const src = reinterpret_cast<T const*>(a.q) +
+                             uint64_t(max(row[n].token, 0)) * a.q_stride +
+                             uint64_t(row[n].head) * uint64_t(a.d);
+#pragma unroll
+        for (int i = 0; i != D / 32; ++i) {
+            int const e = i * 32 + g * 8;
+            q[n][i] = row[n].token >= 0 && e < a.d ? *reinterpret_cast<half8_t const*>(src + e)
+                                                   : half8_t{};
+        }
+#pragma unroll
+        for (int t = 0; t != DT; ++t) o[n][t] = float4_t{0, 0, 0, 0};
+        m[n] = NEG_INF;
+        l[n] = 0;
+    }
+
+    if (lo < hi) {
+        T const* const kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
+        T const* const vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
+        int const      first = lo / 32 * 32;
+        int const      tiles = (hi - first + KT - 1) / KT;
+        int const      ch = tid % CH, cr = tid / CH;  // this thread's chunk and row of a pass
+        bool const     chunk_in = ch * 8 < a.d;
+        half8_t        kr[PASS], vr[PASS];
+        uint32_t       held = 0;  // bit p: the row of pass p has an entry
+
+        int  page = -1, prow = 0;
+        auto look_up = [&](int tile) {  // threads below KT: the page of key tid
+            int const pos = first + tile * KT + tid;
+            page = -1;
+            if (tid < KT && pos >= lo && pos < hi) {
+                int const pi = page_of(a, pos);
+                prow = pos - pi * a.page_size;
+                page = wk.table[pi];
+            }
+        };
+        auto put_entries = [&](int tile) {
+            if (tid < KT) sh.off[tile & 1][tid] = entry_of(a, page, prow);
+        };
+        auto fetch = [&](int tile) {
+            held = 0;
+#pragma unroll
+            for (int p = 0; p != PASS; ++p) {
+                int64_t const at = sh.off[tile & 1][p * M::RPP + cr];
+                if (at >= 0) held |= 1u << p;
+                int64_t const from = (at < 0 ? 0 : at) + (chunk_in ? ch * 8 : 0);
+                kr[p] = *reinterpret_cast<half8_t const*>(kb + from);
+                vr[p] = *reinterpret_cast<half8_t const*>(vb + from);
+            }
+        };
+        auto put_down = [&](int tile, bool edge) {
+            bool bad = false;
+#pragma unroll
+            for (int p = 0; p != PASS; ++p) {
+                int const  r = p * M::RPP + cr;
+                bool const in = (held >> p & 1) && chunk_in;
+                half8_t const kx = in ? kr[p] : half8_t{};
+                half8_t const vx = in ? vr[p] : half8_t{};
+                sh.k[tile & 1][r][ch ^ (r & 15 & (CH - 1))] = kx;
+                sh.v[tile & 1][r][ch ^ ((2 * (r & 7)) & (CH - 1))] = vx;
+                if (edge) {
+                    u32x4_t const u = __builtin_bit_cast(u32x4_t, vx);
+#pragma unroll
+                    for (int i = 0; i != 4; ++i) {
+                        bad |= (u[i] & 0x7c00u) == 0x7c00u || (u[i] & 0x7c000000u) == 0x7c000000u;
+                    }
+                }
+            }
+            if (bad) sh.bad[tile % 3] = 1;
+        };
+        // the least limit of the workgroup's rows decides where values have to be looked at
+        int const all_see = [&] {
+            __syncthreads();  // limit[] is read above
+            if (tid == 0) sh.limit[0] = 0x7fffffff;
+            if (tid < 3) sh.bad[tid] = 0;
+            __syncthreads();
+            if (lane == 0) atomicMin(&sh.limit[0], least);
+            __syncthreads();
+            return __builtin_amdgcn_readfirstlane(sh.limit[0]);
+        }();
+        auto masks = [&](int tile) { return first + tile * KT + KT - 1 > all_see; };
+
+        look_up(0);
+        put_entries(0);
+        look_up(1);
+        put_entries(1);
+        __syncthreads();
+        fetch(0);
+        look_up(2);
+        put_down(0, masks(0));
+        if (tiles > 1) fetch(1);
+        __syncthreads();
+        for (int tile = 0; tile != tiles; ++tile) {
+            int const buf = tile & 1, base = first + tile * KT;
+            // entries of tile + 2: this tile's were read before the last barrier
+            put_entries(tile + 2);
+            look_up(tile + 3);
+            bool const edge = base < lo || base + KT > hi || base + KT - 1 > least;
+            bool const careful = masks(tile) && sh.bad[tile % 3] != 0;
+            if (base <= most) {
+                float4_t s[NT][KT / 16];
+#pragma unroll
+                for (int t = 0; t != KT / 16; ++t) {
+#pragma unroll
+                    for (int n = 0; n != NT; ++n) s[n][t] = float4_t{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i != D / 32; ++i) {
+                        half8_t const kf = sh.k[buf][16 * t + c][(4 * i + g) ^ (c & (CH - 1))];
+#pragma unroll
+                        for (int n = 0; n != NT; ++n) {
+                            s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[n][i], s[n][t], 0,
+                                                                            0, 0);
+                        }
+                    }
+                }
+                half8_t p[NT][KT / 32];
+#pragma unroll
+                for (int n = 0; n != NT; ++n) {
+                    float top = NEG_INF;
+#pragma unroll
+                    for (int t = 0; t != KT / 16; ++t) {
+                        s[n][t] *= a.scale;
+                        if (edge) {
+#pragma unroll
+                            for (int r = 0; r != 4; ++r) {
+                                int const pos = base + 16 * t + 4 * g + r;
+                                if (pos < lo || pos >= hi || pos > row[n].limit) {
+                                    s[n][t][r] = NEG_INF;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int r = 0; r != 4; ++r) top = fmaxf(top, s[n][t][r]);
+                    }
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    float const mn = fmaxf(m[n], top);
+                    float const ref = mn == NEG_INF ? 0.0f : mn;
+                    if (__any(mn > m[n])) {
+                        float const fade = exp2_fast(m[n] - ref);
+                        l[n] *= fade;
+#pragma unroll
+                        for (int t = 0; t != DT; ++t) o[n][t] *= fade;
+                        m[n] = mn;
+                    }
+                    float sum = 0;
+#pragma unroll
+                    for (int t = 0; t != KT / 16; ++t) {
+#pragma unroll
+                        for (int r = 0; r != 4; ++r) {
+                            float const e = exp2_fast(s[n][t][r] - ref);
+                            sum += e;
+                            p[n][t / 2][4 * (t & 1) + r] = T(e);
+                        }
+                    }
+                    l[n] += sum;
+                }
+                // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of
+                // its own element
+                typedef short tr_t __attribute__((ext_vector_type(4)));
+                auto value_frag = [&](int ks, int t) {
+                    union {
+                        tr_t    x[2];
+                        half8_t h;
+                    } f;
+#pragma unroll
+                    for (int half = 0; half != 2; ++half) {
+                        int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
+                        int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
+                        char*     at = reinterpret_cast<char*>(&sh.v[buf][r][chunk]) + (c & 1) * 8;
+                        f.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) tr_t*)(at));
+                    }
+                    return f.h;
+                };
+                if (!careful) {
+#pragma unroll
+                    for (int t = 0; t != DT; ++t) {
+#pragma unroll
+                        for (int ks = 0; ks != KT / 32; ++ks) {
+                            half8_t const vf = value_frag(ks, t);
+#pragma unroll
+                            for (int n = 0; n != NT; ++n) {
+                                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[n][ks],
+                                                                                o[n][t], 0, 0, 0);
+                            }
+                        }
+                    }
+                } else {
+                    // row by row, each with the keys it sees: zero times infinity is no zero
+#pragma unroll
+                    for (int n = 0; n != NT; ++n) {
+                        for (int r = 0; r != 16; ++r) {
+                            int const limit = __shfl(row[n].limit, r);
+#pragma unroll
+                            for (int t = 0; t != DT; ++t) {
+                                float4_t x = {0, 0, 0, 0};
+#pragma unroll
+                                for (int ks = 0; ks != KT / 32; ++ks) {
+                                    half8_t vf = value_frag(ks, t);
+#pragma unroll
+                                    for (int j = 0; j != 8; ++j) {
+                                        int const key = 32 * ks + 16 * (j >> 2) + 4 * g + (j & 3);
+                                        if (base + key > limit) vf[j] = T(0);
+                                    }
+                                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[n][ks], x, 0, 0,
+                                                                              0);
+                                }
+                                if (c == r) o[n][t] += x;
+                            }
+                        }
+                    }
+                }
+            }
+            if (tile + 1 != tiles) put_down(tile + 1, masks(tile + 1));
+            __syncthreads();
+            if (tid == 0) sh.bad[tile % 3] = 0;
+            if (tile + 2 < tiles) fetch(tile + 2);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n != NT; ++n) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (row[n].token < 0) continue;
+        // O^T: elements 16 t + 4 g + r of this lane's row
+        if (wk.direct) {
+            T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(row[n].token) * a.out_stride +
+                           uint64_t(row[n].head) * uint64_t(a.d);
+            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / l[n];
+#pragma unroll
+            for (int t = 0; t != DT; ++t) {
+                int const e = 16 * t + 4 * g;
+                half4_t   y;
+#pragma unroll
+                for (int r = 0; r != 4; ++r) y[r] = T(m[n] == NEG_INF ? 0.0f : o[n][t][r] * inv);
+                if (e < a.d) *reinterpret_cast<half4_t*>(dst + e) = y;
+            }
+        } else {
+            int64_t const at = wk.part + (w * NT + n) * 16 + c;
+#pragma unroll
+            for (int t = 0; t != DT; ++t) {
+                *reinterpret_cast<float4_t*>(a.part_o + at * D + 16 * t + 4 * g) = o[n][t];
+            }
+            if (g == 0) {
+                a.part_ml[at * 2] = m[n];
+                a.part_ml[at * 2 + 1] = l[n];
+            }
+        }
     }
 }
 
@@ -645,17 +1017,18 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
     if (splits <= 0) return;
     int const kvh = head / a.group, hg = head - kvh * a.group;
     int const prow = token * a.group + hg, srow = (token - b) * a.group + hg;
-    int const pslot = prow / ROWS;
-    int const sslot = meta[0] + srow / ROWS * splits;
+    int const pslot = prow / a.prefix_rows;
+    int const sslot = meta[0] + srow / a.own_rows * splits;
     int const parts = a.prefix_splits + splits;
-    int const slots = a.prefix_tiles * a.prefix_splits + a.items;
     auto      place = [&](int i) -> int64_t {
-        int const pre = i < a.prefix_splits;
-        int const slot = pre ? pslot + i * a.prefix_tiles : sslot + i - a.prefix_splits;
-        int const r = pre ? prow % ROWS : srow % ROWS;
+        if (i < a.prefix_splits) {
+            return (int64_t(pslot + i * a.prefix_tiles) * a.h_kv + kvh) * a.prefix_rows +
+                   prow % a.prefix_rows;
+        }
         // stays inside the workspace whatever the device arrays held
-        int const in = min(max(slot, 0), slots - 1);
-        return (int64_t(in) * a.h_kv + kvh) * ROWS + r;
+        int const slot = min(max(sslot + i - a.prefix_splits, 0), a.items - 1);
+        return a.own_base + (int64_t(slot) * a.h_kv + kvh) * a.own_rows +
+               max(srow, 0) % a.own_rows;
     };
     float top = NEG_INF;
     for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[place(i) * 2]);
@@ -690,10 +1063,34 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 template <typename T, int D>
+void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
+{
+    a.parts = parts;
+    uint64_t const units = (parts & 1 ? uint64_t(a.prefix_tiles) * a.prefix_splits : 0) +
+                           (parts & 2 ? a.items : 0);
+    uint32_t const grid = uint32_t(units * a.h_kv);
+    if constexpr (sizeof(T) == 2) {
+        if (rows == many_t<D, 2>::ROWS) {
+            attention_many_kernel<D, 2><<<grid, THREADS, 0, stream>>>(a);
+            return;
+        }
+        if (rows == many_t<D, 1>::ROWS) {
+            attention_many_kernel<D, 1><<<grid, THREADS, 0, stream>>>(a);
+            return;
+        }
+    }
+    attention_few_kernel<T, D><<<grid, THREADS, 0, stream>>>(a);
+}
+
+template <typename T, int D>
 void launch_dim(attention_dev_t const& a, hipStream_t stream)
 {
-    uint64_t const units = uint64_t(a.prefix_tiles) * a.prefix_splits + a.items;
-    attention_kernel<T, D><<<uint32_t(units * a.h_kv), THREADS, 0, stream>>>(a);
+    if (a.prefix_splits != 0 && a.prefix_rows == a.own_rows) {
+        launch_rows<T, D>(a, 3, a.own_rows, stream);
+    } else {
+        if (a.prefix_splits != 0) launch_rows<T, D>(a, 1, a.prefix_rows, stream);
+        launch_rows<T, D>(a, 2, a.own_rows, stream);
+    }
     if (a.prefix_splits != 0 || a.split_target != 0) {
         uint64_t const rows = uint64_t(a.n_tokens) * a.h_kv * a.group;
         attention_join_kernel<T, D><<<uint32_t((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
@@ -713,6 +1110,13 @@ void launch_type(attention_dev_t const& a, hipStream_t stream)
     }
 }
 
+// Rows per tile for `rows` rows that read the same keys.
+uint32_t tile_rows(int dtype, uint64_t rows)
+{
+    if (dtype != ES_KM_F16 || rows <= FEW) return FEW;
+    return rows <= 64 ? 64 : 128;
+}
+
 }  // namespace
 
 attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tokens,
@@ -722,26 +1126,33 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (n_seqs == 0 || n_tokens == 0) return p;
     uint64_t const kv = uint64_t(c.n_kv_heads), group = uint64_t(c.n_heads / c.n_kv_heads);
     uint64_t const rows = uint64_t(n_tokens) * group;
+    uint64_t const seqs = uint64_t(std::min(n_seqs, n_tokens));  // that have tokens, at most
+    uint64_t       part_rows = 0;
     if (shared > 0) {
-        uint64_t const tiles = (rows + ROWS - 1) / ROWS;
+        p.prefix_rows = tile_rows(c.dtype, rows);
+        uint64_t const tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
         uint64_t const want = (512 + tiles * kv - 1) / (tiles * kv);
         uint64_t const most = (shared + 255) / 256;
         uint64_t const splits = std::max<uint64_t>(1, std::min(want, most));
-        uint64_t const chunk = ((shared + splits - 1) / splits + 31) / 32 * 32;
+        uint64_t const chunk = ((shared + splits - 1) / splits + 63) / 64 * 64;
         p.prefix_tiles = uint32_t(tiles);
         p.prefix_chunk = uint32_t(chunk);
         p.prefix_splits = uint32_t((shared + chunk - 1) / chunk);
+        part_rows = tiles * p.prefix_splits * kv * p.prefix_rows;
     }
-    // sum over the sequences with tokens of ceil(tokens * group / ROWS)
-    uint64_t const tiles = uint64_t(std::min(n_seqs, n_tokens)) + rows / ROWS;
+    p.own_base = part_rows;
+    p.own_rows = tile_rows(c.dtype, rows / seqs);
+    // sum over the sequences with tokens of ceil(tokens * group / own_rows)
+    uint64_t const tiles = seqs + rows / p.own_rows;
     uint64_t const fill = 1024 / kv;
     uint64_t const target =
         tiles * kv >= 8192 ? 0 : std::max(fill > tiles ? fill - tiles : 0, (tiles + 1) / 2);
     p.split_target = uint32_t(target);
     p.items = uint32_t(tiles + target);
-    uint64_t const slots = (uint64_t(p.prefix_tiles) * p.prefix_splits + p.items) * kv * ROWS;
-    p.workspace_bytes = up256(slots * uint64_t(padded_dim(c.head_dim)) * 4) + up256(slots * 8) +
-                        up256(uint64_t(n_tokens) * 16);
+    part_rows += p.items * kv * p.own_rows;
+    p.part_rows = part_rows;
+    p.workspace_bytes = up256(part_rows * uint64_t(padded_dim(c.head_dim)) * 4) +
+                        up256(part_rows * 8) + up256(uint64_t(n_tokens) * 16);
     return p;
 }
 
@@ -773,18 +1184,27 @@ void launch_attention(attention_args_t const& g, attention_plan_t const& p, void
     a.d = g.cache.head_dim;
     a.shared = int(g.shared);
     a.scale = g.scale * 1.44269504088896340736f;
+    int shift = 0;
+    while ((1 << shift) < a.page_size) ++shift;
+    // (2^(30+s) + e) / page_size with e < page_size <= 2^s: exact for positions below 2^30
+    a.page_shift = uint32_t(30 + shift);
+    a.page_magic = uint32_t(((1ull << a.page_shift) + uint64_t(a.page_size) - 1) /
+                            uint64_t(a.page_size));
     a.prefix_tiles = int(p.prefix_tiles);
     a.prefix_splits = int(p.prefix_splits);
     a.prefix_chunk = int(p.prefix_chunk);
+    a.prefix_rows = int(p.prefix_rows);
     a.split_target = int(p.split_target);
     a.items = int(p.items);
-    uint64_t const slots = (uint64_t(p.prefix_tiles) * p.prefix_splits + p.items) *
-                           uint64_t(a.h_kv) * ROWS;
+    a.own_rows = int(p.own_rows);
+    a.own_base = int64_t(p.own_base);
+    a.direct = p.prefix_splits == 0;
+    a.parts = 0;
     char* const    ws = static_cast<char*>(workspace);
+    uint64_t const o_bytes = up256(p.part_rows * uint64_t(padded_dim(a.d)) * 4);
     a.part_o = reinterpret_cast<float*>(ws);
-    uint64_t const o_bytes = up256(slots * uint64_t(padded_dim(a.d)) * 4);
     a.part_ml = reinterpret_cast<float*>(ws + o_bytes);
-    a.part_meta = reinterpret_cast<int*>(ws + o_bytes + up256(slots * 8));
+    a.part_meta = reinterpret_cast<int*>(ws + o_bytes + up256(p.part_rows * 8));
     if (g.cache.dtype == ES_KM_F16) {
         launch_type<_Float16>(a, stream);
     } else {

@@ -58,11 +58,15 @@ struct attention_args_t {
 
 // How one call is cut into workgroups; a function of the sizes the host knows.
 struct attention_plan_t {
+    uint32_t prefix_rows = 0;    // rows per tile, shared positions
     uint32_t prefix_tiles = 0;   // row tiles over all tokens of the batch
     uint32_t prefix_splits = 0;  // cuts of the shared positions
     uint32_t prefix_chunk = 0;   // positions per cut
-    uint32_t split_target = 0;   // cuts of the sequences' own positions, over the whole batch
+    uint32_t own_rows = 0;       // rows per tile, the sequences' own positions
+    uint32_t split_target = 0;   // cuts of the own positions, over the whole batch
     uint32_t items = 0;          // upper bound of (row tile, cut) pairs of the own positions
+    uint64_t own_base = 0;       // rows of partial results before the own positions'
+    uint64_t part_rows = 0;      // rows of partial results
     uint64_t workspace_bytes = 0;
 };
 
