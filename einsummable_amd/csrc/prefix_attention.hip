@@ -117,7 +117,7 @@ struct row_t {
 struct deal_t {
     long long total[WAVES];
     int       before[WAVES];
-    int       found[4];  // sequence, item within it, first slot, cuts
+    int       found[8];  // sequence, item within it, first item, cuts, offsets, length
 };
 
 template <int ROWS>
@@ -140,6 +140,16 @@ __device__ inline row_t row_of(attention_dev_t const& a, work_t const& k, int co
     row.head = kvh * a.group + r - j * a.group;
     row.limit = at;
     return row;
+}
+
+// Workgroups go to the eight XCDs in turn.  The heads of one unit (a row tile and a cut) stay on
+// one XCD: together they read whole rows of the cache, while one head per XCD would ask its L2
+// for 256 bytes every n_kv_heads * 256, which few of its channels hold.
+__device__ inline void unit_of_block(attention_dev_t const& a, int& unit, int& kvh)
+{
+    int const xcd = int(blockIdx.x) & 7, i = int(blockIdx.x) >> 3;
+    kvh = i % a.h_kv;
+    unit = i / a.h_kv * 8 + xcd;
 }
 
 // Finds the workgroup's work; false: there is none.  `limit` holds ROWS ints.
@@ -181,15 +191,19 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
     int const item = unit - prefix_units;
     int const run = (a.n_seqs + THREADS - 1) / THREADS;
     int const s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
+    if (item >= a.items) return false;
     if (tid == 0) sh.found[0] = -1;
     long long total = 0;
+    int  sb = 0, se = 0, slen = 0, tiles = 0, steps = 0;
     auto tiles_steps = [&](int s, int& tiles, int& steps) {
-        int const b = max(a.offsets[s], 0), e = min(a.offsets[s + 1], a.n_tokens);
-        int const len = min(a.lens[s], reach);
+        sb = a.offsets[s];
+        se = a.offsets[s + 1];
+        slen = a.lens[s];
+        int const b = max(sb, 0), e = min(se, a.n_tokens);
+        int const len = min(slen, reach);
         tiles = e > b ? ((e - b) * a.group + ROWS - 1) / ROWS : 0;
         steps = len > a.shared ? (len + KS - 1) / KS - a.shared / KS : 0;
     };
-    int tiles = 0, steps = 0;
     for (int s = s0; s < s1; ++s) {
         tiles_steps(s, tiles, steps);
         total += (long long)tiles * steps;
@@ -231,6 +245,9 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
                 sh.found[1] = item - start;
                 sh.found[2] = start;
                 sh.found[3] = splits;
+                sh.found[4] = sb;
+                sh.found[5] = se;
+                sh.found[6] = slen;
                 break;
             }
             start += tiles * splits;
@@ -241,10 +258,10 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
     if (s < 0) return false;
     int const splits = sh.found[3];
     int const tile = sh.found[1] / splits, split = sh.found[1] - tile * splits;
-    k.b = max(a.offsets[s], 0);
-    k.e = min(a.offsets[s + 1], a.n_tokens);
-    k.end = a.offsets[s + 1];
-    k.len = a.lens[s];
+    k.b = max(sh.found[4], 0);
+    k.e = min(sh.found[5], a.n_tokens);
+    k.end = sh.found[5];
+    k.len = sh.found[6];
     k.whole = false;
     k.part = a.own_base + (int64_t(item) * a.h_kv + kvh) * ROWS;
     k.direct = splits == 1 && a.direct;
@@ -289,48 +306,70 @@ struct core_t<_Float16, D> {
 
     static __device__ int key_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
 
+    // PAD: d is below D.  Loads are unconditional (a branch around each would make it wait for
+    // the one before); elements beyond d come from the row's start and are zeroed.
+    template <bool PAD>
     __device__ void load_q(_Float16 const* row, int g, int d)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
-            int const e = c * 32 + g * 8;
-            q[c] = row && e < d ? *reinterpret_cast<half8_t const*>(row + e) : half8_t{};
+            int const  e = c * 32 + g * 8;
+            bool const in = !PAD || e < d;
+            q[c] = *reinterpret_cast<half8_t const*>(row + (in ? e : 0));
+            if (PAD && !in) q[c] = half8_t{};
         }
     }
-    // element offsets of the two keys this lane loads of K, the eight of V
+    // element offsets of the two keys this lane loads of K, the eight of V; negative ones (no
+    // such entry) read the cache's first, to be masked by the caller
+    template <bool PAD>
     __device__ void load(_Float16 const* kb, _Float16 const* vb, int64_t const* off, int c, int g,
                          int d)
     {
+        int64_t ok[2], ov[KL];
+#pragma unroll
+        for (int t = 0; t != 2; ++t) ok[t] = off[16 * t + c];
+#pragma unroll
+        for (int j = 0; j != KL; ++j) ov[j] = off[key_of(j, g)];
 #pragma unroll
         for (int t = 0; t != 2; ++t) {
-            int64_t const o = off[16 * t + c];
-            _Float16 const* p = kb + (o < 0 ? 0 : o);
+            _Float16 const* p = kb + max(ok[t], int64_t(0));
 #pragma unroll
             for (int i = 0; i != QC; ++i) {
                 int const e = i * 32 + g * 8;
-                k[t][i] = e < d ? *reinterpret_cast<half8_t const*>(p + e) : half8_t{};
+                k[t][i] = *reinterpret_cast<half8_t const*>(p + (!PAD || e < d ? e : 0));
             }
         }
+        constexpr int N = DV < 8 ? DV : 8;  // d is a multiple of 8
+        typedef uint32_t vec_t __attribute__((ext_vector_type(N / 2)));
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
-            int64_t const o = off[key_of(j, g)];
-            _Float16 const* p = vb + (o < 0 ? 0 : o) + c * DV;
-            constexpr int N = DV < 8 ? DV : 8;  // d is a multiple of 8
+            _Float16 const* p = vb + max(ov[j], int64_t(0));
 #pragma unroll
             for (int e = 0; e != DV; e += N) {
-                if (c * DV + e < d) {
-                    __builtin_memcpy(&v[j].h[e], __builtin_assume_aligned(p + e, N * 2), N * 2);
-                } else {
+                bool const  in = !PAD || c * DV + e < d;
+                vec_t const x = *reinterpret_cast<vec_t const*>(p + (in ? c * DV + e : 0));
 #pragma unroll
-                    for (int i = 0; i != N; ++i) v[j].h[e + i] = 0;
+                for (int i = 0; i != N / 2; ++i) v[j].u[e / 2 + i] = x[i];
+            }
+        }
+        if (PAD) {
+#pragma unroll
+            for (int i = 0; i != QC; ++i) {
+                if (i * 32 + g * 8 >= d) k[0][i] = k[1][i] = half8_t{};
+            }
+#pragma unroll
+            for (int j = 0; j != KL; ++j) {
+#pragma unroll
+                for (int i = 0; i != DV / 2; ++i) {
+                    v[j].u[i] = c * DV + 2 * i < d ? v[j].u[i] : 0;
                 }
             }
         }
     }
-    __device__ void drop_key(int j)
+    __device__ void keep_key(int j, bool keep)
     {
 #pragma unroll
-        for (int i = 0; i != DV / 2; ++i) v[j].u[i] = 0;
+        for (int i = 0; i != DV / 2; ++i) v[j].u[i] = keep ? v[j].u[i] : 0;
     }
     __device__ bool not_finite(int j) const
     {
@@ -404,40 +443,57 @@ struct core_t<float, D> {
 
     static __device__ int key_of(int j, int g) { return 4 * g + j; }
 
+    template <bool PAD>
     __device__ void load_q(float const* row, int g, int d)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
-            int const e = c * 16 + g * 4;
-            q[c] = row && e < d ? *reinterpret_cast<float4_t const*>(row + e) : float4_t{};
+            int const  e = c * 16 + g * 4;
+            bool const in = !PAD || e < d;
+            q[c] = *reinterpret_cast<float4_t const*>(row + (in ? e : 0));
+            if (PAD && !in) q[c] = float4_t{};
         }
     }
+    template <bool PAD>
     __device__ void load(float const* kb, float const* vb, int64_t const* off, int c, int g, int d)
     {
         int64_t const ok = off[c];
-        float const*  p = kb + (ok < 0 ? 0 : ok);
+        int64_t       ov[KL];
+#pragma unroll
+        for (int j = 0; j != KL; ++j) ov[j] = off[key_of(j, g)];
+        float const* p = kb + max(ok, int64_t(0));
 #pragma unroll
         for (int i = 0; i != QC; ++i) {
             int const e = i * 16 + g * 4;
-            k[i] = e < d ? *reinterpret_cast<float4_t const*>(p + e) : float4_t{};
+            k[i] = *reinterpret_cast<float4_t const*>(p + (!PAD || e < d ? e : 0));
         }
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
-            int64_t const o = off[key_of(j, g)];
-            float const*  pv = vb + (o < 0 ? 0 : o) + c * DV;
+            float const* pv = vb + max(ov[j], int64_t(0));
 #pragma unroll
             for (int e = 0; e != DV; e += 4) {
-                float4_t const x = c * DV + e < d ? *reinterpret_cast<float4_t const*>(pv + e)
-                                                  : float4_t{};
+                bool const     in = !PAD || c * DV + e < d;
+                float4_t const x = *reinterpret_cast<float4_t const*>(pv + (in ? c * DV + e : 0));
 #pragma unroll
                 for (int i = 0; i != 4; ++i) v[j][e + i] = x[i];
             }
         }
+        if (PAD) {
+#pragma unroll
+            for (int i = 0; i != QC; ++i) {
+                if (i * 16 + g * 4 >= d) k[i] = float4_t{};
+            }
+#pragma unroll
+            for (int j = 0; j != KL; ++j) {
+#pragma unroll
+                for (int e = 0; e != DV; ++e) v[j][e] = c * DV + e < d ? v[j][e] : 0.0f;
+            }
+        }
     }
-    __device__ void drop_key(int j)
+    __device__ void keep_key(int j, bool keep)
     {
 #pragma unroll
-        for (int i = 0; i != DV; ++i) v[j][i] = 0;
+        for (int i = 0; i != DV; ++i) v[j][i] = keep ? v[j][i] : 0.0f;
     }
     __device__ bool not_finite(int j) const
     {
@@ -496,7 +552,7 @@ struct few_shared_t {
 };
 
 // The workgroup's keys against the tile's rows; steps w, w + WAVES, ...
-template <typename T, int D>
+template <typename T, int D, bool PAD>
 __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const& wk, row_t const& row,
                            int least, int kvh, float4_t* o, float& m, float& l)
 {
@@ -508,10 +564,11 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
     T const* const       kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
     T const* const       vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
     core                 x;
-    x.load_q(row.token < 0 ? nullptr
-                           : reinterpret_cast<T const*>(a.q) + uint64_t(row.token) * a.q_stride +
-                                 uint64_t(row.head) * uint64_t(a.d),
-             g, a.d);
+    // a column without a row computes what nobody stores
+    x.template load_q<PAD>(reinterpret_cast<T const*>(a.q) +
+                               uint64_t(max(row.token, 0)) * a.q_stride +
+                               uint64_t(row.head) * uint64_t(a.d),
+                           g, a.d);
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
@@ -536,7 +593,9 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         look_up(base + WAVES * KS);
-        x.load(kb, vb, off, c, g, a.d);
+        x.template load<PAD>(kb, vb, off, c, g, a.d);
+        // all of the step's loads go out before the first is waited for
+        __builtin_amdgcn_sched_barrier(0);
         float s[KL];
         x.scores(s);
         bool const edge = holes || base + KS - 1 > seen_by_all;
@@ -546,8 +605,8 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             for (int j = 0; j != KL; ++j) {
                 int const  key = core::key_of(j, g);
                 bool const hole = off[key] < 0;
-                if (hole) x.drop_key(j);
-                if (hole || base + key > row.limit) masked |= 1u << j;
+                x.keep_key(j, !hole);
+                masked |= hole || base + key > row.limit ? 1u << j : 0;
             }
         }
         float top = NEG_INF;
@@ -600,17 +659,16 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
     l += __shfl_xor(l, 32);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PAD>
 __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kernel(attention_dev_t a)
 {
     __shared__ few_shared_t<T, D> sh;
     int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
     int const c = lane & 15, g = lane >> 4;
-    int const kvh = int(blockIdx.x) % a.h_kv;
-    work_t    wk;
-    if (!deal<FEW, core_t<T, D>::KS>(a, sh.deal, sh.limit, int(blockIdx.x) / a.h_kv, kvh, wk)) {
-        return;
-    }
+    int       unit, kvh;
+    unit_of_block(a, unit, kvh);
+    work_t wk;
+    if (!deal<FEW, core_t<T, D>::KS>(a, sh.deal, sh.limit, unit, kvh, wk)) return;
     row_t const row = row_of<FEW>(a, wk, sh.limit, kvh, c);
     int         least = row.limit;
 #pragma unroll
@@ -621,7 +679,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 #pragma unroll
     for (int t = 0; t != DV; ++t) o[t] = float4_t{0, 0, 0, 0};
     float m = NEG_INF, l = 0;
-    if (wk.lo < wk.hi) attend_few<T, D>(a, sh.off[w], wk, row, least, kvh, o, m, l);
+    if (wk.lo < wk.hi) attend_few<T, D, PAD>(a, sh.off[w], wk, row, least, kvh, o, m, l);
 
     // join the wavefronts
     if (g == 0) {
@@ -671,10 +729,12 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
                 T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(otoken) * a.out_stride +
                                uint64_t(ohead) * uint64_t(a.d) + h * DJ + oe;
                 float const inv = otop == NEG_INF ? 0.0f : 1.0f / sum;
+                // PER divides 8, and 8 divides d: all of them or none
+                typedef T vec_t __attribute__((ext_vector_type(PER)));
+                vec_t     z;
 #pragma unroll
-                for (int e = 0; e != PER; ++e) {
-                    if (h * DJ + oe + e < a.d) dst[e] = T(otop == NEG_INF ? 0.0f : y[e] * inv);
-                }
+                for (int e = 0; e != PER; ++e) z[e] = T(otop == NEG_INF ? 0.0f : y[e] * inv);
+                if (h * DJ + oe < a.d) *reinterpret_cast<vec_t*>(dst) = z;
             } else {
                 float* const dst = a.part_o + (wk.part + orow) * D + h * DJ + oe;
 #pragma unroll
@@ -697,10 +757,10 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 // the row: K by row % 16 (a fragment read takes one chunk of 16 rows), V by 2 (row % 8) (a
 // transposing read takes 32 bytes of four rows).  Two tiles alternate: while one is worked on the
 // next is on its way from global memory to registers, to be put down before the barrier.
-template <int D, int NT>
+template <int D, int NT, int KT_ = D == 64 ? 64 : 32>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
-    static constexpr int KT = D == 256 ? 32 : 64;
+    static constexpr int KT = KT_;
     static constexpr int CH = D / 8;                   // chunks per row
     static constexpr int PASS = KT * CH / THREADS;     // chunks per thread, of K and of V each
     static constexpr int RPP = THREADS / CH;           // rows per pass
@@ -724,9 +784,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
     int const tid = int(threadIdx.x), lane = tid & 63;
     int const w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int const c = lane & 15, g = lane >> 4;
-    int const kvh = int(blockIdx.x) % a.h_kv;
-    work_t    wk;
-    if (!deal<ROWS, 32>(a, sh.deal, sh.limit, int(blockIdx.x) / a.h_kv, kvh, wk)) return;
+    int       unit, kvh;
+    unit_of_block(a, unit, kvh);
+    work_t wk;
+    if (!deal<ROWS, 32>(a, sh.deal, sh.limit, unit, kvh, wk)) return;
     row_t row[NT];
     int   least = 0x7fffffff, most = -1;
 #pragma unroll
@@ -756,8 +817,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
 #pragma unroll
         for (int i = 0; i != D / 32; ++i) {
             int const e = i * 32 + g * 8;
-            q[n][i] = row[n].token >= 0 && e < a.d ? *reinterpret_cast<half8_t const*>(src + e)
-                                                   : half8_t{};
+            q[n][i] = *reinterpret_cast<half8_t const*>(src + (e < a.d ? e : 0));
+            if (e >= a.d) q[n][i] = half8_t{};
         }
 #pragma unroll
         for (int t = 0; t != DT; ++t) o[n][t] = float4_t{0, 0, 0, 0};
@@ -1038,17 +1099,37 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
     float         y[PER], sum = 0;
 #pragma unroll
     for (int e = 0; e != PER; ++e) y[e] = 0;
-    if (top != NEG_INF) {
-        for (int i = 0; i != parts; ++i) {
-            int64_t const at = place(i);
-            float const   m = a.part_ml[at * 2];
-            if (m == NEG_INF) continue;  // a cut without keys for this row
-            float const f = exp2_fast(m - top);
-            sum += a.part_ml[at * 2 + 1] * f;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        // lane i: the place and the weight of cut i0 + i; none without keys for this row
+        bool const    in = i0 + lane < parts;
+        int64_t const at = in ? place(i0 + lane) : 0;
+        float const   mi = in ? a.part_ml[at * 2] : NEG_INF;
+        float const   li = in ? a.part_ml[at * 2 + 1] : 0.0f;
+        float const   f = mi == NEG_INF ? 0.0f : exp2_fast(mi - top);
+        sum += mi == NEG_INF ? 0.0f : li * f;
+        constexpr int U = 8;  // cuts in flight
+        int const     n = min(parts - i0, 64);
+        for (int i = 0; i < n; i += U) {
+            float x[U][PER], fi[U];
 #pragma unroll
-            for (int e = 0; e != PER; ++e) y[e] += a.part_o[at * D + lane * PER + e] * f;
+            for (int u = 0; u != U; ++u) {
+                int const     from = min(i + u, n - 1);
+                int64_t const p = __shfl(at, from);
+                fi[u] = i + u < n ? __shfl(f, from) : 0.0f;
+#pragma unroll
+                for (int e = 0; e != PER; ++e) {
+                    x[u][e] = fi[u] != 0.0f ? a.part_o[p * D + lane * PER + e] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u != U; ++u) {
+#pragma unroll
+                for (int e = 0; e != PER; ++e) y[e] += x[u][e] * fi[u];
+            }
         }
     }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     T* const    dst = reinterpret_cast<T*>(a.out) + uint64_t(token) * a.out_stride +
                    uint64_t(head) * uint64_t(a.d) + lane * PER;
     float const inv = top == NEG_INF ? 0.0f : 1.0f / sum;
@@ -1068,7 +1149,7 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
     a.parts = parts;
     uint64_t const units = (parts & 1 ? uint64_t(a.prefix_tiles) * a.prefix_splits : 0) +
                            (parts & 2 ? a.items : 0);
-    uint32_t const grid = uint32_t(units * a.h_kv);
+    uint32_t const grid = uint32_t((units + 7) / 8 * 8 * a.h_kv);
     if constexpr (sizeof(T) == 2) {
         if (rows == many_t<D, 2>::ROWS) {
             attention_many_kernel<D, 2><<<grid, THREADS, 0, stream>>>(a);
@@ -1079,7 +1160,11 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
             return;
         }
     }
-    attention_few_kernel<T, D><<<grid, THREADS, 0, stream>>>(a);
+    if (a.d == D) {
+        attention_few_kernel<T, D, false><<<grid, THREADS, 0, stream>>>(a);
+    } else {
+        attention_few_kernel<T, D, true><<<grid, THREADS, 0, stream>>>(a);
+    }
 }
 
 template <typename T, int D>
