@@ -57,7 +57,8 @@ struct attention_dev_t {
     int         n_seqs, n_tokens, max_pages, page_size;
     int         h_kv, group, d;
     int         shared;
-    float       scale;  // of the scores, times log2(e)
+    float       scale;   // of the scores, times log2(e); positive
+    float       q_sign;  // -1, 0 or 1, multiplied into q: the sign of the caller's scale
     uint32_t    page_magic, page_shift;
     int         prefix_tiles, prefix_splits, prefix_chunk, prefix_rows;
     int         split_target;
@@ -309,13 +310,13 @@ struct core_t<_Float16, D> {
     // PAD: d is below D.  Loads are unconditional (a branch around each would make it wait for
     // the one before); elements beyond d come from the row's start and are zeroed.
     template <bool PAD>
-    __device__ void load_q(_Float16 const* row, int g, int d)
+    __device__ void load_q(_Float16 const* row, int g, int d, float sign)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
             int const  e = c * 32 + g * 8;
             bool const in = !PAD || e < d;
-            q[c] = *reinterpret_cast<half8_t const*>(row + (in ? e : 0));
+            q[c] = *reinterpret_cast<half8_t const*>(row + (in ? e : 0)) * _Float16(sign);
             if (PAD && !in) q[c] = half8_t{};
         }
     }
@@ -444,13 +445,13 @@ struct core_t<float, D> {
     static __device__ int key_of(int j, int g) { return 4 * g + j; }
 
     template <bool PAD>
-    __device__ void load_q(float const* row, int g, int d)
+    __device__ void load_q(float const* row, int g, int d, float sign)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
             int const  e = c * 16 + g * 4;
             bool const in = !PAD || e < d;
-            q[c] = *reinterpret_cast<float4_t const*>(row + (in ? e : 0));
+            q[c] = *reinterpret_cast<float4_t const*>(row + (in ? e : 0)) * sign;
             if (PAD && !in) q[c] = float4_t{};
         }
     }
@@ -537,6 +538,24 @@ struct core_t<float, D> {
     }
 };
 
+// Takes the largest score of a step into a row's reference m (what exponents are taken relative
+// to) and returns the reference to use, 0 while nothing was seen.  The reference need not be the
+// maximum: it is raised, and what was summed so far scaled down, only where a score passes it by
+// 2^8, which leaves p below 2^8 and f16's relative precision as it is.
+template <int N>
+__device__ inline float raise(float top, float& m, float& l, float4_t* o)
+{
+    if (__any(top > m + 8.0f)) {
+        float const mn = fmaxf(m, top);
+        float const fade = exp2_fast(m - (mn == NEG_INF ? 0.0f : mn));
+        l *= fade;
+#pragma unroll
+        for (int t = 0; t != N; ++t) o[t] *= fade;
+        m = mn;
+    }
+    return m == NEG_INF ? 0.0f : m;
+}
+
 // ------------------------------------------------------------------------------ few rows
 
 constexpr int FEW = 16;
@@ -568,7 +587,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
     x.template load_q<PAD>(reinterpret_cast<T const*>(a.q) +
                                uint64_t(max(row.token, 0)) * a.q_stride +
                                uint64_t(row.head) * uint64_t(a.d),
-                           g, a.d);
+                           g, a.d, a.q_sign);
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
@@ -612,25 +631,19 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
         float top = NEG_INF;
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
-            s[j] = masked >> j & 1 ? NEG_INF : s[j] * a.scale;
+            s[j] = masked >> j & 1 ? NEG_INF : s[j];
             top = fmaxf(top, s[j]);
         }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        float const mn = fmaxf(m, top);
-        // nothing seen yet: any finite reference will do
-        float const ref = mn == NEG_INF ? 0.0f : mn;
-        float const fade = exp2_fast(m - ref);
+        float const ref = raise<DV>(top * a.scale, m, l, o);
         float       sum = 0;
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
-            s[j] = exp2_fast(s[j] - ref);
+            s[j] = exp2_fast(s[j] * a.scale - ref);
             sum += s[j];
         }
-        l = l * fade + sum;
-        m = mn;
-#pragma unroll
-        for (int t = 0; t != DV; ++t) o[t] *= fade;
+        l += sum;
         // Zero times an infinity or NaN is no zero: where a row may not see a key whose values
         // are not finite, the rows are taken one by one, each with the keys it sees.
         bool careful = false;
@@ -757,7 +770,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 // the row: K by row % 16 (a fragment read takes one chunk of 16 rows), V by 2 (row % 8) (a
 // transposing read takes 32 bytes of four rows).  Two tiles alternate: while one is worked on the
 // next is on its way from global memory to registers, to be put down before the barrier.
-template <int D, int NT, int KT_ = D == 64 ? 64 : 32>
+template <int D, int NT, int KT_ = D == 256 ? 32 : 64>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
     static constexpr int KT = KT_;
@@ -769,7 +782,10 @@ struct many_t {
         deal_t   deal;
         int      limit[ROWS];
         int64_t  off[2][KT];
-        int      bad[3];  // of a tile modulo 3: reset a barrier before it is set again
+        uint8_t  hole[2][KT];
+        // of a tile modulo 3 (reset a barrier before they are set again): 1, a value that is not
+        // finite was replaced; 2, a position has no page
+        int      flags[3];
         half8_t  k[2][KT][CH], v[2][KT][CH];
     };
 };
@@ -817,7 +833,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
 #pragma unroll
         for (int i = 0; i != D / 32; ++i) {
             int const e = i * 32 + g * 8;
-            q[n][i] = *reinterpret_cast<half8_t const*>(src + (e < a.d ? e : 0));
+            q[n][i] = *reinterpret_cast<half8_t const*>(src + (e < a.d ? e : 0)) * T(a.q_sign);
             if (e >= a.d) q[n][i] = half8_t{};
         }
 #pragma unroll
@@ -860,31 +876,50 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
                 vr[p] = *reinterpret_cast<half8_t const*>(vb + from);
             }
         };
-        auto put_down = [&](int tile, bool edge) {
+        // Zero times an infinity or NaN is no zero: where some row may not see a key of the tile,
+        // values that are not finite are put down as zeros, and added afterwards to the rows that
+        // see them.
+        auto put_down = [&](int tile, bool masked) {
             bool bad = false;
 #pragma unroll
             for (int p = 0; p != PASS; ++p) {
                 int const  r = p * M::RPP + cr;
                 bool const in = (held >> p & 1) && chunk_in;
                 half8_t const kx = in ? kr[p] : half8_t{};
-                half8_t const vx = in ? vr[p] : half8_t{};
-                sh.k[tile & 1][r][ch ^ (r & 15 & (CH - 1))] = kx;
-                sh.v[tile & 1][r][ch ^ ((2 * (r & 7)) & (CH - 1))] = vx;
-                if (edge) {
-                    u32x4_t const u = __builtin_bit_cast(u32x4_t, vx);
+                half8_t       vx = in ? vr[p] : half8_t{};
+                if (masked) {
 #pragma unroll
-                    for (int i = 0; i != 4; ++i) {
-                        bad |= (u[i] & 0x7c00u) == 0x7c00u || (u[i] & 0x7c000000u) == 0x7c000000u;
+                    for (int i = 0; i != 8; ++i) {
+                        if (!(vx[i] - vx[i] == T(0))) {
+                            vx[i] = T(0);
+                            bad = true;
+                        }
                     }
                 }
+                sh.k[tile & 1][r][ch ^ (r & 15 & (CH - 1))] = kx;
+                sh.v[tile & 1][r][ch ^ ((2 * (r & 7)) & (CH - 1))] = vx;
             }
-            if (bad) sh.bad[tile % 3] = 1;
+            if (bad) atomicOr(&sh.flags[tile % 3], 1);
+            if (held != (1u << PASS) - 1 && ch == 0) {
+#pragma unroll
+                for (int p = 0; p != PASS; ++p) {
+                    int const  r = p * M::RPP + cr, pos = first + tile * KT + r;
+                    bool const hole = !(held >> p & 1);
+                    if (hole && pos >= lo && pos < hi) atomicOr(&sh.flags[tile % 3], 2);
+                }
+            }
+            if (ch == 0) {
+#pragma unroll
+                for (int p = 0; p != PASS; ++p) {
+                    sh.hole[tile & 1][p * M::RPP + cr] = !(held >> p & 1);
+                }
+            }
         };
         // the least limit of the workgroup's rows decides where values have to be looked at
         int const all_see = [&] {
             __syncthreads();  // limit[] is read above
             if (tid == 0) sh.limit[0] = 0x7fffffff;
-            if (tid < 3) sh.bad[tid] = 0;
+            if (tid < 3) sh.flags[tid] = 0;
             __syncthreads();
             if (lane == 0) atomicMin(&sh.limit[0], least);
             __syncthreads();
@@ -907,8 +942,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
             // entries of tile + 2: this tile's were read before the last barrier
             put_entries(tile + 2);
             look_up(tile + 3);
-            bool const edge = base < lo || base + KT > hi || base + KT - 1 > least;
-            bool const careful = masks(tile) && sh.bad[tile % 3] != 0;
+            int const  flags = __builtin_amdgcn_readfirstlane(sh.flags[tile % 3]);
+            bool const holes = flags & 2, careful = flags & 1;
+            bool const edge = holes || base < lo || base + KT > hi || base + KT - 1 > least;
             if (base <= most) {
                 float4_t s[NT][KT / 16];
 #pragma unroll
@@ -928,39 +964,43 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
                 half8_t p[NT][KT / 32];
 #pragma unroll
                 for (int n = 0; n != NT; ++n) {
-                    float top = NEG_INF;
+                    if (edge) {
 #pragma unroll
-                    for (int t = 0; t != KT / 16; ++t) {
-                        s[n][t] *= a.scale;
-                        if (edge) {
+                        for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
                             for (int r = 0; r != 4; ++r) {
                                 int const pos = base + 16 * t + 4 * g + r;
-                                if (pos < lo || pos >= hi || pos > row[n].limit) {
+                                if (pos < lo || pos > min(hi - 1, row[n].limit)) {
                                     s[n][t][r] = NEG_INF;
                                 }
                             }
                         }
+                        // a page that does not exist
+                        if (holes) {
+#pragma unroll
+                            for (int t = 0; t != KT / 16; ++t) {
+#pragma unroll
+                                for (int r = 0; r != 4; ++r) {
+                                    if (sh.hole[buf][16 * t + 4 * g + r]) s[n][t][r] = NEG_INF;
+                                }
+                            }
+                        }
+                    }
+                    float top = NEG_INF;
+#pragma unroll
+                    for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
                         for (int r = 0; r != 4; ++r) top = fmaxf(top, s[n][t][r]);
                     }
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
-                    float const mn = fmaxf(m[n], top);
-                    float const ref = mn == NEG_INF ? 0.0f : mn;
-                    if (__any(mn > m[n])) {
-                        float const fade = exp2_fast(m[n] - ref);
-                        l[n] *= fade;
-#pragma unroll
-                        for (int t = 0; t != DT; ++t) o[n][t] *= fade;
-                        m[n] = mn;
-                    }
-                    float sum = 0;
+                    float const ref = raise<DT>(top * a.scale, m[n], l[n], o[n]);
+                    float       sum = 0;
 #pragma unroll
                     for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
                         for (int r = 0; r != 4; ++r) {
-                            float const e = exp2_fast(s[n][t][r] - ref);
+                            float const e = exp2_fast(s[n][t][r] * a.scale - ref);
                             sum += e;
                             p[n][t / 2][4 * (t & 1) + r] = T(e);
                         }
@@ -970,55 +1010,50 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
                 // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of
                 // its own element
                 typedef short tr_t __attribute__((ext_vector_type(4)));
-                auto value_frag = [&](int ks, int t) {
-                    union {
-                        tr_t    x[2];
-                        half8_t h;
-                    } f;
 #pragma unroll
-                    for (int half = 0; half != 2; ++half) {
-                        int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
-                        int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
-                        char*     at = reinterpret_cast<char*>(&sh.v[buf][r][chunk]) + (c & 1) * 8;
-                        f.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) tr_t*)(at));
-                    }
-                    return f.h;
-                };
-                if (!careful) {
+                for (int t = 0; t != DT; ++t) {
 #pragma unroll
-                    for (int t = 0; t != DT; ++t) {
+                    for (int ks = 0; ks != KT / 32; ++ks) {
+                        union {
+                            tr_t    x[2];
+                            half8_t h;
+                        } vf;
 #pragma unroll
-                        for (int ks = 0; ks != KT / 32; ++ks) {
-                            half8_t const vf = value_frag(ks, t);
+                        for (int half = 0; half != 2; ++half) {
+                            int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
+                            int const chunk =
+                                (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
+                            char* at = reinterpret_cast<char*>(&sh.v[buf][r][chunk]) + (c & 1) * 8;
+                            vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) tr_t*)(at));
+                        }
 #pragma unroll
-                            for (int n = 0; n != NT; ++n) {
-                                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[n][ks],
-                                                                                o[n][t], 0, 0, 0);
-                            }
+                        for (int n = 0; n != NT; ++n) {
+                            o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, p[n][ks], o[n][t],
+                                                                            0, 0, 0);
                         }
                     }
-                } else {
-                    // row by row, each with the keys it sees: zero times infinity is no zero
+                }
+                // what put_down() replaced by zeros, for the rows that see it
+                if (careful) {
+                    for (int i = 0; i != KT; ++i) {
+                        int const pos = base + i;
+                        if (pos < lo || pos >= hi) continue;
+                        int const     pi = page_of(a, pos);
+                        int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
+                        if (at < 0) continue;
 #pragma unroll
-                    for (int n = 0; n != NT; ++n) {
-                        for (int r = 0; r != 16; ++r) {
-                            int const limit = __shfl(row[n].limit, r);
+                        for (int t = 0; t != DT; ++t) {
 #pragma unroll
-                            for (int t = 0; t != DT; ++t) {
-                                float4_t x = {0, 0, 0, 0};
+                            for (int r = 0; r != 4; ++r) {
+                                int const e = 16 * t + 4 * g + r;
+                                if (e >= a.d) continue;
+                                float const x = float(vb[at + e]);
+                                if (x - x == 0.0f) continue;
 #pragma unroll
-                                for (int ks = 0; ks != KT / 32; ++ks) {
-                                    half8_t vf = value_frag(ks, t);
-#pragma unroll
-                                    for (int j = 0; j != 8; ++j) {
-                                        int const key = 32 * ks + 16 * (j >> 2) + 4 * g + (j & 3);
-                                        if (base + key > limit) vf[j] = T(0);
-                                    }
-                                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[n][ks], x, 0, 0,
-                                                                              0);
+                                for (int n = 0; n != NT; ++n) {
+                                    if (pos <= row[n].limit) o[n][t][r] += x;
                                 }
-                                if (c == r) o[n][t] += x;
                             }
                         }
                     }
@@ -1026,7 +1061,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
             }
             if (tile + 1 != tiles) put_down(tile + 1, masks(tile + 1));
             __syncthreads();
-            if (tid == 0) sh.bad[tile % 3] = 0;
+            if (tid == 0) sh.flags[tile % 3] = 0;
             if (tile + 2 < tiles) fetch(tile + 2);
         }
     }
@@ -1151,9 +1186,11 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
                            (parts & 2 ? a.items : 0);
     uint32_t const grid = uint32_t((units + 7) / 8 * 8 * a.h_kv);
     if constexpr (sizeof(T) == 2) {
-        if (rows == many_t<D, 2>::ROWS) {
-            attention_many_kernel<D, 2><<<grid, THREADS, 0, stream>>>(a);
-            return;
+        if constexpr (D <= 128) {
+            if (rows == many_t<D, 2>::ROWS) {
+                attention_many_kernel<D, 2><<<grid, THREADS, 0, stream>>>(a);
+                return;
+            }
         }
         if (rows == many_t<D, 1>::ROWS) {
             attention_many_kernel<D, 1><<<grid, THREADS, 0, stream>>>(a);
@@ -1195,11 +1232,12 @@ void launch_type(attention_dev_t const& a, hipStream_t stream)
     }
 }
 
-// Rows per tile for `rows` rows that read the same keys.
-uint32_t tile_rows(int dtype, uint64_t rows)
+// Rows per tile for `rows` rows that read the same keys.  32 rows of 256 elements per wavefront
+// would not fit its registers.
+uint32_t tile_rows(es_km_kv_cache_t const& c, uint64_t rows)
 {
-    if (dtype != ES_KM_F16 || rows <= FEW) return FEW;
-    return rows <= 64 ? 64 : 128;
+    if (c.dtype != ES_KM_F16 || rows <= FEW) return FEW;
+    return rows <= 64 || c.head_dim > 128 ? 64 : 128;
 }
 
 }  // namespace
@@ -1213,10 +1251,16 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     uint64_t const rows = uint64_t(n_tokens) * group;
     uint64_t const seqs = uint64_t(std::min(n_seqs, n_tokens));  // that have tokens, at most
     uint64_t       part_rows = 0;
+    p.own_rows = tile_rows(c, rows / seqs);
+    // A prefix of its own pays where rows of several sequences fill a tile together.  Sequences
+    // that fill tiles by themselves read it through their own tables.
+    if (p.own_rows == (c.head_dim > 128 ? 64 : 128)) shared = 0;
+    p.shared = uint32_t(shared);
     if (shared > 0) {
-        p.prefix_rows = tile_rows(c.dtype, rows);
+        p.prefix_rows = tile_rows(c, rows);
         uint64_t const tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
-        uint64_t const want = (512 + tiles * kv - 1) / (tiles * kv);
+        uint64_t W = 512; if (getenv("X_PRE")) W = atoi(getenv("X_PRE"));
+        uint64_t const want = (W + tiles * kv - 1) / (tiles * kv);
         uint64_t const most = (shared + 255) / 256;
         uint64_t const splits = std::max<uint64_t>(1, std::min(want, most));
         uint64_t const chunk = ((shared + splits - 1) / splits + 63) / 64 * 64;
@@ -1226,10 +1270,14 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
         part_rows = tiles * p.prefix_splits * kv * p.prefix_rows;
     }
     p.own_base = part_rows;
-    p.own_rows = tile_rows(c.dtype, rows / seqs);
     // sum over the sequences with tokens of ceil(tokens * group / own_rows)
-    uint64_t const tiles = seqs + rows / p.own_rows;
-    uint64_t const fill = 1024 / kv;
+    uint64_t tiles = seqs + (rows - seqs) / p.own_rows;
+    // where a tile holds at least two groups, a sequence's first token adds no second tile
+    if (2 * group <= p.own_rows + 1) {
+        tiles = std::min(tiles, seqs + (rows - seqs * group) / (p.own_rows - group + 1));
+    }
+    uint64_t fill = 1024 / kv;
+    if (getenv("X_FILL")) fill = atoi(getenv("X_FILL")) / kv;
     uint64_t const target =
         tiles * kv >= 8192 ? 0 : std::max(fill > tiles ? fill - tiles : 0, (tiles + 1) / 2);
     p.split_target = uint32_t(target);
@@ -1267,8 +1315,9 @@ void launch_attention(attention_args_t const& g, attention_plan_t const& p, void
     a.h_kv = g.cache.n_kv_heads;
     a.group = g.cache.n_heads / g.cache.n_kv_heads;
     a.d = g.cache.head_dim;
-    a.shared = int(g.shared);
-    a.scale = g.scale * 1.44269504088896340736f;
+    a.shared = int(p.shared);
+    a.scale = g.scale == 0.0f ? 1.0f : __builtin_fabsf(g.scale) * 1.44269504088896340736f;
+    a.q_sign = g.scale == 0.0f ? 0.0f : g.scale < 0.0f ? -1.0f : 1.0f;
     int shift = 0;
     while ((1 << shift) < a.page_size) ++shift;
     // (2^(30+s) + e) / page_size with e < page_size <= 2^s: exact for positions below 2^30

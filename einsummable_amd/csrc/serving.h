@@ -58,6 +58,7 @@ struct attention_args_t {
 
 // How one call is cut into workgroups; a function of the sizes the host knows.
 struct attention_plan_t {
+    uint32_t shared = 0;         // positions treated as shared
     uint32_t prefix_rows = 0;    // rows per tile, shared positions
     uint32_t prefix_tiles = 0;   // row tiles over all tokens of the batch
     uint32_t prefix_splits = 0;  // cuts of the shared positions

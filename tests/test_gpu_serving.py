@@ -216,8 +216,10 @@ def test_attention_lengths_of_zero_and_one_and_shorter_than_the_prefix(km, dtype
 
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("shared", [0, 65])
-def test_attention_ignores_what_masked_places_hold(km, dtype, shared):
-    b = Paged(23, dtype, 4, 2, 64, 8, [6, 1, 20], [shared + 6, shared + 19, shared + 41], shared)
+@pytest.mark.parametrize("more", [0, 80])
+def test_attention_ignores_what_masked_places_hold(km, dtype, shared, more):
+    b = Paged(23, dtype, 4, 2, 64, 8, [6 + more, 1 + more, 20],
+              [shared + 6 + more, shared + 19 + more, shared + 41], shared)
     clean = run_attention(km, b)
     for bad in (np.nan, np.inf, -np.inf):
         for which in (b.k, b.v):
@@ -251,6 +253,23 @@ def test_attention_leaves_out_pages_that_do_not_exist(km):
     b.table[2, :] = 1 << 30          # none at all: zeros
     got = run_attention(km, b)
     assert not got[5].any()
+    # the same with tiles of many rows, in shared and in own positions
+    b = Paged(33, F16, 4, 2, 64, 8, [40, 1, 70], [140, 101, 190], shared=70)
+    b.table[:, 3] = -1
+    b.table[0, 12] = b.n_pages
+    b.table[2, 9:] = -7
+    run_attention(km, b)
+    b = Paged(34, F16, 4, 2, 128, 8, [1] * 40, [90] * 40, shared=70)
+    b.table[:, 5] = -1
+    b.table[7, 10] = -1
+    run_attention(km, b)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_attention_scale_of_zero_and_below(km, dtype, scale):
+    run_attention(km, Paged(35, dtype, 4, 2, 64, 8, [1, 3], [70, 33], shared=20), scale=scale)
+    run_attention(km, Paged(36, dtype, 4, 2, 64, 8, [50, 3], [70, 33], shared=20), scale=scale)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
