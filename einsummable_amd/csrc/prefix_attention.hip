@@ -766,36 +766,73 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 
 // ------------------------------------------------------------------------------ many rows
 
-// f16 only.  A tile of KT keys lies in LDS as rows of D elements, 16-byte chunks XOR-swizzled with
+// What rows without an entry, and elements beyond head_dim, are loaded from.
+__device__ __align__(16) uint32_t const attention_zeros[4] = {0, 0, 0, 0};
+
+// 64 lanes x 16 bytes from each lane's address to LDS at lds + 16 * lane.
+__device__ __forceinline__ void load_to_lds_16(void const* from, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds), "v"(from)
+                 : "memory");
+}
+
+__device__ __forceinline__ void load_to_lds_4(void const* from, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :
+                 : "s"(lds), "v"(from)
+                 : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(void const* p)
+{
+    return __builtin_amdgcn_readfirstlane(
+        uint32_t(uintptr_t((__attribute__((address_space(3))) char const*)(p))));
+}
+
+// f16 only.  Tiles of KT keys lie in LDS as rows of D elements, 16-byte chunks XOR-swizzled with
 // the row: K by row % 16 (a fragment read takes one chunk of 16 rows), V by 2 (row % 8) (a
-// transposing read takes 32 bytes of four rows).  Two tiles alternate: while one is worked on the
-// next is on its way from global memory to registers, to be put down before the barrier.
-template <int D, int NT, int KT_ = D == 256 ? 32 : 64>
+// transposing read takes 32 bytes of four rows); neither read has bank conflicts.  The loads go
+// from global memory straight to LDS, NS - 1 tiles ahead, one barrier per tile.  Where a
+// position's entry lies is worked out for a window of 256 positions at a time, a position per
+// thread; the page numbers of the next window come through LDS as well, several tiles ahead, so
+// no wait for them drains the tiles in flight.
+template <int D, int NT>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
-    static constexpr int KT = KT_;
-    static constexpr int CH = D / 8;                   // chunks per row
-    static constexpr int PASS = KT * CH / THREADS;     // chunks per thread, of K and of V each
-    static constexpr int RPP = THREADS / CH;           // rows per pass
+    static constexpr int KT = 32;
+    static constexpr int NS = D == 256 ? 3 : 4;
+    static constexpr int CH = D / 8;             // chunks per row
+    static constexpr int RPL = 64 / CH;          // rows per load instruction
+    static constexpr int LPT = KT / RPL / WAVES; // load instructions per wavefront and tile, of K
     static constexpr int DT = D / 16;
+    static constexpr int WINDOW = 256, TPW = WINDOW / KT;
     struct shared_t {
-        deal_t   deal;
-        int      limit[ROWS];
-        int64_t  off[2][KT];
-        uint8_t  hole[2][KT];
-        // of a tile modulo 3 (reset a barrier before they are set again): 1, a value that is not
-        // finite was replaced; 2, a position has no page
-        int      flags[3];
-        half8_t  k[2][KT][CH], v[2][KT][CH];
+        deal_t  deal;
+        int     limit[ROWS];
+        int64_t entry[2][WINDOW];
+        int     page[WINDOW];
+        int     holes;     // some position has no page
+        int     flags[2];  // a tile's values were not all finite
+        half8_t k[NS][KT][CH], v[NS][KT][CH];
     };
 };
 
 template <int D, int NT>
-__global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_dev_t a)
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kernel(attention_dev_t a)
 {
     typedef many_t<D, NT> M;
     typedef _Float16      T;
-    constexpr int         ROWS = M::ROWS, KT = M::KT, CH = M::CH, PASS = M::PASS, DT = M::DT;
+    constexpr int         ROWS = M::ROWS, KT = M::KT, CH = M::CH, DT = M::DT, NS = M::NS;
+    constexpr int         LPT = M::LPT;
     __shared__ typename M::shared_t sh;
     int const tid = int(threadIdx.x), lane = tid & 63;
     int const w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -847,223 +884,208 @@ __global__ __launch_bounds__(THREADS, 2) void attention_many_kernel(attention_de
         T const* const vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
         int const      first = lo / 32 * 32;
         int const      tiles = (hi - first + KT - 1) / KT;
-        int const      ch = tid % CH, cr = tid / CH;  // this thread's chunk and row of a pass
-        bool const     chunk_in = ch * 8 < a.d;
-        half8_t        kr[PASS], vr[PASS];
-        uint32_t       held = 0;  // bit p: the row of pass p has an entry
 
-        int  page = -1, prow = 0;
-        auto look_up = [&](int tile) {  // threads below KT: the page of key tid
-            int const pos = first + tile * KT + tid;
-            page = -1;
-            if (tid < KT && pos >= lo && pos < hi) {
-                int const pi = page_of(a, pos);
-                prow = pos - pi * a.page_size;
-                page = wk.table[pi];
-            }
+        // this thread's position of window n
+        auto position = [&](int n) { return first + n * M::WINDOW + tid; };
+        auto ask_page = [&](int n) {  // page numbers of window n, to LDS
+            int const pos = position(n);
+            load_to_lds_4(wk.table + (pos >= lo && pos < hi ? page_of(a, pos) : page_of(a, lo)),
+                          lds_address(&sh.page[w * 64]));
         };
-        auto put_entries = [&](int tile) {
-            if (tid < KT) sh.off[tile & 1][tid] = entry_of(a, page, prow);
+        auto put_entry = [&](int n) {
+            int const pos = position(n);
+            int64_t   at = -1;
+            if (pos >= lo && pos < hi) {
+                at = entry_of(a, sh.page[tid], pos - page_of(a, pos) * a.page_size);
+                if (at < 0) sh.holes = 1;
+            }
+            sh.entry[n & 1][tid] = at;
         };
-        auto fetch = [&](int tile) {
-            held = 0;
+        // this lane's row and chunk in a load instruction
+        int const lrow = lane / CH, lpos = lane % CH;
+        auto      load_tile = [&](int tile) {
+            int64_t const* const entry =
+                &sh.entry[tile / M::TPW & 1][tile % M::TPW * KT];
+            int const slot = tile % NS;
 #pragma unroll
-            for (int p = 0; p != PASS; ++p) {
-                int64_t const at = sh.off[tile & 1][p * M::RPP + cr];
-                if (at >= 0) held |= 1u << p;
-                int64_t const from = (at < 0 ? 0 : at) + (chunk_in ? ch * 8 : 0);
-                kr[p] = *reinterpret_cast<half8_t const*>(kb + from);
-                vr[p] = *reinterpret_cast<half8_t const*>(vb + from);
-            }
-        };
-        // Zero times an infinity or NaN is no zero: where some row may not see a key of the tile,
-        // values that are not finite are put down as zeros, and added afterwards to the rows that
-        // see them.
-        auto put_down = [&](int tile, bool masked) {
-            bool bad = false;
-#pragma unroll
-            for (int p = 0; p != PASS; ++p) {
-                int const  r = p * M::RPP + cr;
-                bool const in = (held >> p & 1) && chunk_in;
-                half8_t const kx = in ? kr[p] : half8_t{};
-                half8_t       vx = in ? vr[p] : half8_t{};
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i != 8; ++i) {
-                        if (!(vx[i] - vx[i] == T(0))) {
-                            vx[i] = T(0);
-                            bad = true;
-                        }
-                    }
-                }
-                sh.k[tile & 1][r][ch ^ (r & 15 & (CH - 1))] = kx;
-                sh.v[tile & 1][r][ch ^ ((2 * (r & 7)) & (CH - 1))] = vx;
-            }
-            if (bad) atomicOr(&sh.flags[tile % 3], 1);
-            if (held != (1u << PASS) - 1 && ch == 0) {
-#pragma unroll
-                for (int p = 0; p != PASS; ++p) {
-                    int const  r = p * M::RPP + cr, pos = first + tile * KT + r;
-                    bool const hole = !(held >> p & 1);
-                    if (hole && pos >= lo && pos < hi) atomicOr(&sh.flags[tile % 3], 2);
-                }
-            }
-            if (ch == 0) {
-#pragma unroll
-                for (int p = 0; p != PASS; ++p) {
-                    sh.hole[tile & 1][p * M::RPP + cr] = !(held >> p & 1);
-                }
+            for (int i = 0; i != LPT; ++i) {
+                int const     r0 = (i * WAVES + w) * M::RPL;
+                int const     r = r0 + lrow;
+                int64_t const at = entry[r];
+                int const     kc = lpos ^ (r & 15 & (CH - 1));
+                int const     vc = lpos ^ ((2 * (r & 7)) & (CH - 1));
+                void const*   zeros = attention_zeros;
+                load_to_lds_16(at >= 0 && kc * 8 < a.d ? kb + at + kc * 8 : zeros,
+                                    lds_address(&sh.k[slot][r0][0]));
+                load_to_lds_16(at >= 0 && vc * 8 < a.d ? vb + at + vc * 8 : zeros,
+                                    lds_address(&sh.v[slot][r0][0]));
             }
         };
         // the least limit of the workgroup's rows decides where values have to be looked at
-        int const all_see = [&] {
-            __syncthreads();  // limit[] is read above
-            if (tid == 0) sh.limit[0] = 0x7fffffff;
-            if (tid < 3) sh.flags[tid] = 0;
-            __syncthreads();
-            if (lane == 0) atomicMin(&sh.limit[0], least);
-            __syncthreads();
-            return __builtin_amdgcn_readfirstlane(sh.limit[0]);
-        }();
-        auto masks = [&](int tile) { return first + tile * KT + KT - 1 > all_see; };
-
-        look_up(0);
-        put_entries(0);
-        look_up(1);
-        put_entries(1);
+        __syncthreads();  // limit[] is read above
+        if (tid == 0) {
+            sh.limit[0] = 0x7fffffff;
+            sh.holes = sh.flags[0] = sh.flags[1] = 0;
+        }
+        ask_page(0);
+        wait_loads<0>();
         __syncthreads();
-        fetch(0);
-        look_up(2);
-        put_down(0, masks(0));
-        if (tiles > 1) fetch(1);
+        if (lane == 0) atomicMin(&sh.limit[0], least);
+        put_entry(0);
         __syncthreads();
-        for (int tile = 0; tile != tiles; ++tile) {
-            int const buf = tile & 1, base = first + tile * KT;
-            // entries of tile + 2: this tile's were read before the last barrier
-            put_entries(tile + 2);
-            look_up(tile + 3);
-            int const  flags = __builtin_amdgcn_readfirstlane(sh.flags[tile % 3]);
-            bool const holes = flags & 2, careful = flags & 1;
+        int const all_see = __builtin_amdgcn_readfirstlane(sh.limit[0]);
+        ask_page(1);
+#pragma unroll
+        for (int i = 0; i != NS - 1; ++i) {
+            // beyond the last tile too: the wait below counts instructions (their entries are -1)
+            load_tile(i);
+        }
+        for (int tile = 0; tile < tiles; ++tile) {
+            int const slot = tile % NS, base = first + tile * KT;
+            wait_loads<2 * LPT*(NS - 2)>();
+            __syncthreads();
+            bool const masked = base + KT - 1 > all_see;
+            int        careful = 0;
+            if (masked) {
+                // Zero times an infinity or NaN is no zero: where some row may not see a key of
+                // the tile, values that are not finite become zeros, and are added afterwards to
+                // the rows that see them.
+                bool bad = false;
+                for (int i = tid; i < KT * CH; i += THREADS) {
+                    half8_t& x = sh.v[slot][i / CH][i % CH];
+                    half8_t  y = x;
+                    bool     any = false;
+#pragma unroll
+                    for (int e = 0; e != 8; ++e) {
+                        if (!(y[e] - y[e] == T(0))) {
+                            y[e] = T(0);
+                            any = true;
+                        }
+                    }
+                    if (any) {
+                        x = y;
+                        bad = true;
+                    }
+                }
+                if (tid == 0) sh.flags[(tile + 1) & 1] = 0;
+                if (bad) sh.flags[tile & 1] = 1;
+                __syncthreads();
+                careful = __builtin_amdgcn_readfirstlane(sh.flags[tile & 1]);
+            }
+            {
+                // tile + NS - 1 goes where the last one was; windows are prepared on the way
+                int const j = tile + NS - 1;
+                load_tile(j);
+                int const n = j / M::TPW, at = j % M::TPW;
+                if (at == M::TPW - 2) put_entry(n + 1);
+                if (at == M::TPW - 1) ask_page(n + 2);
+            }
+            if (base > most) continue;
+            bool const holes = sh.holes != 0;
             bool const edge = holes || base < lo || base + KT > hi || base + KT - 1 > least;
-            if (base <= most) {
-                float4_t s[NT][KT / 16];
+            float4_t   s[NT][KT / 16];
+#pragma unroll
+            for (int t = 0; t != KT / 16; ++t) {
+#pragma unroll
+                for (int n = 0; n != NT; ++n) s[n][t] = float4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i != D / 32; ++i) {
+                    half8_t const kf = sh.k[slot][16 * t + c][(4 * i + g) ^ (c & (CH - 1))];
+#pragma unroll
+                    for (int n = 0; n != NT; ++n) {
+                        s[n][t] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[n][i], s[n][t], 0, 0, 0);
+                    }
+                }
+            }
+            if (edge) {
+                int64_t const* const entry = &sh.entry[tile / M::TPW & 1][tile % M::TPW * KT];
 #pragma unroll
                 for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
-                    for (int n = 0; n != NT; ++n) s[n][t] = float4_t{0, 0, 0, 0};
-#pragma unroll
-                    for (int i = 0; i != D / 32; ++i) {
-                        half8_t const kf = sh.k[buf][16 * t + c][(4 * i + g) ^ (c & (CH - 1))];
+                    for (int r = 0; r != 4; ++r) {
+                        int const  key = 16 * t + 4 * g + r;
+                        bool const none = entry[key] < 0;  // not among the positions, or no page
 #pragma unroll
                         for (int n = 0; n != NT; ++n) {
-                            s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[n][i], s[n][t], 0,
-                                                                            0, 0);
+                            if (none || base + key > row[n].limit) s[n][t][r] = NEG_INF;
                         }
                     }
                 }
-                half8_t p[NT][KT / 32];
+            }
+            half8_t p[NT][KT / 32];
 #pragma unroll
-                for (int n = 0; n != NT; ++n) {
-                    if (edge) {
+            for (int n = 0; n != NT; ++n) {
+                float top = NEG_INF;
 #pragma unroll
-                        for (int t = 0; t != KT / 16; ++t) {
+                for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
-                            for (int r = 0; r != 4; ++r) {
-                                int const pos = base + 16 * t + 4 * g + r;
-                                if (pos < lo || pos > min(hi - 1, row[n].limit)) {
-                                    s[n][t][r] = NEG_INF;
-                                }
-                            }
-                        }
-                        // a page that does not exist
-                        if (holes) {
+                    for (int r = 0; r != 4; ++r) top = fmaxf(top, s[n][t][r]);
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                float const ref = raise<DT>(top * a.scale, m[n], l[n], o[n]);
+                float       sum = 0;
 #pragma unroll
-                            for (int t = 0; t != KT / 16; ++t) {
+                for (int t = 0; t != KT / 16; ++t) {
 #pragma unroll
-                                for (int r = 0; r != 4; ++r) {
-                                    if (sh.hole[buf][16 * t + 4 * g + r]) s[n][t][r] = NEG_INF;
-                                }
-                            }
-                        }
+                    for (int r = 0; r != 4; ++r) {
+                        float const e = exp2_fast(s[n][t][r] * a.scale - ref);
+                        sum += e;
+                        p[n][t / 2][4 * (t & 1) + r] = T(e);
                     }
-                    float top = NEG_INF;
+                }
+                l[n] += sum;
+            }
+            // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of its
+            // own element
+            typedef short tr_t __attribute__((ext_vector_type(4)));
 #pragma unroll
-                    for (int t = 0; t != KT / 16; ++t) {
+            for (int t = 0; t != DT; ++t) {
 #pragma unroll
-                        for (int r = 0; r != 4; ++r) top = fmaxf(top, s[n][t][r]);
+                for (int ks = 0; ks != KT / 32; ++ks) {
+                    union {
+                        tr_t    x[2];
+                        half8_t h;
+                    } vf;
+#pragma unroll
+                    for (int half = 0; half != 2; ++half) {
+                        int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
+                        int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
+                        char* at = reinterpret_cast<char*>(&sh.v[slot][r][chunk]) + (c & 1) * 8;
+                        vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) tr_t*)(at));
                     }
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    float const ref = raise<DT>(top * a.scale, m[n], l[n], o[n]);
-                    float       sum = 0;
 #pragma unroll
-                    for (int t = 0; t != KT / 16; ++t) {
+                    for (int n = 0; n != NT; ++n) {
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, p[n][ks], o[n][t], 0,
+                                                                        0, 0);
+                    }
+                }
+            }
+            if (careful) {
+                for (int i = 0; i != KT; ++i) {
+                    int64_t const at = sh.entry[tile / M::TPW & 1][tile % M::TPW * KT + i];
+                    if (at < 0) continue;
+#pragma unroll
+                    for (int t = 0; t != DT; ++t) {
 #pragma unroll
                         for (int r = 0; r != 4; ++r) {
-                            float const e = exp2_fast(s[n][t][r] * a.scale - ref);
-                            sum += e;
-                            p[n][t / 2][4 * (t & 1) + r] = T(e);
-                        }
-                    }
-                    l[n] += sum;
-                }
-                // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of
-                // its own element
-                typedef short tr_t __attribute__((ext_vector_type(4)));
+                            int const e = 16 * t + 4 * g + r;
+                            if (e >= a.d) continue;
+                            float const x = float(vb[at + e]);
+                            if (x - x == 0.0f) continue;
 #pragma unroll
-                for (int t = 0; t != DT; ++t) {
-#pragma unroll
-                    for (int ks = 0; ks != KT / 32; ++ks) {
-                        union {
-                            tr_t    x[2];
-                            half8_t h;
-                        } vf;
-#pragma unroll
-                        for (int half = 0; half != 2; ++half) {
-                            int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
-                            int const chunk =
-                                (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
-                            char* at = reinterpret_cast<char*>(&sh.v[buf][r][chunk]) + (c & 1) * 8;
-                            vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) tr_t*)(at));
-                        }
-#pragma unroll
-                        for (int n = 0; n != NT; ++n) {
-                            o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, p[n][ks], o[n][t],
-                                                                            0, 0, 0);
-                        }
-                    }
-                }
-                // what put_down() replaced by zeros, for the rows that see it
-                if (careful) {
-                    for (int i = 0; i != KT; ++i) {
-                        int const pos = base + i;
-                        if (pos < lo || pos >= hi) continue;
-                        int const     pi = page_of(a, pos);
-                        int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
-                        if (at < 0) continue;
-#pragma unroll
-                        for (int t = 0; t != DT; ++t) {
-#pragma unroll
-                            for (int r = 0; r != 4; ++r) {
-                                int const e = 16 * t + 4 * g + r;
-                                if (e >= a.d) continue;
-                                float const x = float(vb[at + e]);
-                                if (x - x == 0.0f) continue;
-#pragma unroll
-                                for (int n = 0; n != NT; ++n) {
-                                    if (pos <= row[n].limit) o[n][t][r] += x;
-                                }
+                            for (int n = 0; n != NT; ++n) {
+                                if (base + i <= row[n].limit) o[n][t][r] += x;
                             }
                         }
                     }
                 }
             }
-            if (tile + 1 != tiles) put_down(tile + 1, masks(tile + 1));
-            __syncthreads();
-            if (tid == 0) sh.flags[tile % 3] = 0;
-            if (tile + 2 < tiles) fetch(tile + 2);
         }
+        // nothing may still be on its way to LDS when the workgroup ends
+        wait_loads<0>();
     }
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
