@@ -75,11 +75,45 @@ constexpr float NEG_INF = -__builtin_huge_valf();
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ inline long long wave_sum(long long v)
+// Inclusive sums over the 64 lanes.
+__device__ inline int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // row_bcast:31
+    return v;
+}
+
+// Sum over the 64 lanes, in every lane; the same additions whatever the wavefront.
+__device__ inline float wave_sum(float v)
 {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
+}
+
+// Maximum and sum over the four lanes that share a column (lane % 16).
+__device__ inline float column_max(float x)
+{
+    uint32_t u = __builtin_bit_cast(uint32_t, x);
+    auto     r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    // by way of variables: a bit cast of r[1] itself reads r[0]
+    uint32_t lo = r[0], hi = r[1];
+    u = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, lo),
+                                           __builtin_bit_cast(float, hi)));
+    r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    lo = r[0];
+    hi = r[1];
+    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+
+__device__ inline float column_sum(float x)
+{
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
 }
 
 // pos / page_size, exact below 2^30 positions
@@ -116,9 +150,9 @@ struct row_t {
 };
 
 struct deal_t {
-    long long total[WAVES];
-    int       before[WAVES];
-    int       found[8];  // sequence, item within it, first item, cuts, offsets, length
+    float total[WAVES];
+    int   before[WAVES];
+    int   found[8];  // sequence, item within it, first item, cuts, offsets, length
 };
 
 template <int ROWS>
@@ -188,14 +222,11 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
         return true;
     }
     // The cuts of all sequences, numbered through: tiles_s * splits_s each, where a cut holds
-    // `chunk` steps.  A thread adds up a run of sequences.
+    // `chunk` steps.  Up to 64 sequences every wavefront adds up for itself, one per lane;
+    // more are dealt to the threads in runs.
     int const item = unit - prefix_units;
-    int const run = (a.n_seqs + THREADS - 1) / THREADS;
-    int const s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
     if (item >= a.items) return false;
-    if (tid == 0) sh.found[0] = -1;
-    long long total = 0;
-    int  sb = 0, se = 0, slen = 0, tiles = 0, steps = 0;
+    int  sb = 0, se = 0, slen = 0;
     auto tiles_steps = [&](int s, int& tiles, int& steps) {
         sb = a.offsets[s];
         se = a.offsets[s + 1];
@@ -205,64 +236,90 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
         tiles = e > b ? ((e - b) * a.group + ROWS - 1) / ROWS : 0;
         steps = len > a.shared ? (len + KS - 1) / KS - a.shared / KS : 0;
     };
-    for (int s = s0; s < s1; ++s) {
-        tiles_steps(s, tiles, steps);
-        total += (long long)tiles * steps;
-    }
-    long long const ws = wave_sum(total);
-    if (lane == 0) sh.total[w] = ws;
-    __syncthreads();
-    long long all = 0;
-#pragma unroll
-    for (int i = 0; i != WAVES; ++i) all += sh.total[i];
-    // a multiple of four steps: one for each wavefront that takes them in turn
-    int chunk = 0x3fffffff;
-    if (a.split_target > 0) {
-        long long const per = (all + a.split_target - 1) / a.split_target;
-        chunk = int(max((long long)WAVES, (per + WAVES - 1) / WAVES * WAVES));
-    }
-    int mine = 0;
-    for (int s = s0; s < s1; ++s) {
-        if (run > 1) tiles_steps(s, tiles, steps);
-        mine += tiles * max(1, (steps + chunk - 1) / chunk);
-    }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        int const up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
-    }
-    if (lane == 63) sh.before[w] = incl;
-    __syncthreads();
-    int start = incl - mine;
-#pragma unroll
-    for (int i = 0; i != WAVES; ++i) start += i < w ? sh.before[i] : 0;
-    if (item >= start && item < start + mine) {
-        for (int s = s0; s < s1; ++s) {
-            if (run > 1) tiles_steps(s, tiles, steps);
-            int const splits = max(1, (steps + chunk - 1) / chunk);
-            if (item < start + tiles * splits) {
-                sh.found[0] = s;
-                sh.found[1] = item - start;
-                sh.found[2] = start;
-                sh.found[3] = splits;
-                sh.found[4] = sb;
-                sh.found[5] = se;
-                sh.found[6] = slen;
-                break;
-            }
-            start += tiles * splits;
+    // Steps per cut, a multiple of four: one for each wavefront that takes them in turn.  The sum
+    // is taken in fp32, so 2^-10 of it and one step are added: the cuts never number more than the
+    // grid was made for.
+    auto steps_per_cut = [&](float all) {
+        if (a.split_target <= 0) return 0x3fffffff;
+        float const per = all / float(a.split_target) * (1.0f + 0x1p-10f) + 1.0f;
+        return int(fminf(per, 1e9f)) / WAVES * WAVES + WAVES;
+    };
+    auto cuts = [](int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); };
+    int  s, index, first_item, splits, chunk, seq_b, seq_e, seq_len;
+    if (a.n_seqs <= 64) {
+        int tiles = 0, steps = 0;
+        if (lane < a.n_seqs) tiles_steps(lane, tiles, steps);
+        chunk = __builtin_amdgcn_readfirstlane(
+            steps_per_cut(wave_sum(float(tiles) * float(steps))));
+        int const      each = cuts(steps, chunk);
+        int const      mine = tiles * each;
+        int const      start = wave_scan(mine) - mine;
+        uint64_t const here = __ballot(item >= start && item < start + mine);
+        if (here == 0) return false;
+        s = __ffsll((unsigned long long)here) - 1;
+        first_item = __builtin_amdgcn_readlane(start, s);
+        splits = __builtin_amdgcn_readlane(each, s);
+        seq_b = __builtin_amdgcn_readlane(sb, s);
+        seq_e = __builtin_amdgcn_readlane(se, s);
+        seq_len = __builtin_amdgcn_readlane(slen, s);
+        index = item - first_item;
+    } else {
+        int const run = (a.n_seqs + THREADS - 1) / THREADS;
+        int const s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
+        if (tid == 0) sh.found[0] = -1;
+        float total = 0;
+        int   tiles = 0, steps = 0;
+        for (int i = s0; i < s1; ++i) {
+            tiles_steps(i, tiles, steps);
+            total += float(tiles) * float(steps);
         }
+        total = wave_sum(total);
+        if (lane == 0) sh.total[w] = total;
+        __syncthreads();
+        chunk = steps_per_cut(sh.total[0] + sh.total[1] + sh.total[2] + sh.total[3]);
+        int mine = 0;
+        for (int i = s0; i < s1; ++i) {
+            if (run > 1) tiles_steps(i, tiles, steps);
+            mine += tiles * cuts(steps, chunk);
+        }
+        int const incl = wave_scan(mine);
+        if (lane == 63) sh.before[w] = incl;
+        __syncthreads();
+        int start = incl - mine;
+#pragma unroll
+        for (int i = 0; i != WAVES; ++i) start += i < w ? sh.before[i] : 0;
+        if (item >= start && item < start + mine) {
+            for (int i = s0; i < s1; ++i) {
+                if (run > 1) tiles_steps(i, tiles, steps);
+                int const each = cuts(steps, chunk);
+                if (item < start + tiles * each) {
+                    sh.found[0] = i;
+                    sh.found[1] = item - start;
+                    sh.found[2] = start;
+                    sh.found[3] = each;
+                    sh.found[4] = sb;
+                    sh.found[5] = se;
+                    sh.found[6] = slen;
+                    break;
+                }
+                start += tiles * each;
+            }
+        }
+        __syncthreads();
+        s = __builtin_amdgcn_readfirstlane(sh.found[0]);
+        if (s < 0) return false;
+        index = __builtin_amdgcn_readfirstlane(sh.found[1]);
+        first_item = __builtin_amdgcn_readfirstlane(sh.found[2]);
+        splits = __builtin_amdgcn_readfirstlane(sh.found[3]);
+        seq_b = __builtin_amdgcn_readfirstlane(sh.found[4]);
+        seq_e = __builtin_amdgcn_readfirstlane(sh.found[5]);
+        seq_len = __builtin_amdgcn_readfirstlane(sh.found[6]);
     }
-    __syncthreads();
-    int const s = sh.found[0];
-    if (s < 0) return false;
-    int const splits = sh.found[3];
-    int const tile = sh.found[1] / splits, split = sh.found[1] - tile * splits;
-    k.b = max(sh.found[4], 0);
-    k.e = min(sh.found[5], a.n_tokens);
-    k.end = sh.found[5];
-    k.len = sh.found[6];
+    int const tile = index / splits, split = index - tile * splits;
+    k.b = max(seq_b, 0);
+    k.e = min(seq_e, a.n_tokens);
+    k.end = seq_e;
+    k.len = seq_len;
     k.whole = false;
     k.part = a.own_base + (int64_t(item) * a.h_kv + kvh) * ROWS;
     k.direct = splits == 1 && a.direct;
@@ -273,7 +330,7 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
         int const first = k.b + k.r0 / a.group;
         for (int t = first + tid; t <= last; t += THREADS) {
             int* const meta = a.part_meta + 4 * t;
-            meta[0] = sh.found[2];
+            meta[0] = first_item;
             meta[1] = k.direct ? 0 : splits;
             meta[2] = k.b;
         }
@@ -634,8 +691,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             s[j] = masked >> j & 1 ? NEG_INF : s[j];
             top = fmaxf(top, s[j]);
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = column_max(top);
         float const ref = raise<DV>(top * a.scale, m, l, o);
         float       sum = 0;
 #pragma unroll
@@ -668,8 +724,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
         }
     }
     // the four lanes of a column hold sums over different keys
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = column_sum(l);
 }
 
 template <typename T, int D, bool PAD>
@@ -767,7 +822,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 // ------------------------------------------------------------------------------ many rows
 
 // What rows without an entry, and elements beyond head_dim, are loaded from.
-__device__ __align__(16) uint32_t const attention_zeros[4] = {0, 0, 0, 0};
+__device__ __align__(16) uint32_t const attention_zeros[128] = {0};
 
 // 64 lanes x 16 bytes from each lane's address to LDS at lds + 16 * lane.
 __device__ __forceinline__ void load_to_lds_16(void const* from, uint32_t lds)
@@ -805,6 +860,10 @@ __device__ __forceinline__ uint32_t lds_address(void const* p)
 // position's entry lies is worked out for a window of 256 positions at a time, a position per
 // thread; the page numbers of the next window come through LDS as well, several tiles ahead, so
 // no wait for them drains the tiles in flight.
+//
+// The scores of tile i + 1 are computed in the iteration that turns those of tile i into weights:
+// the exponentials take the vector unit about as long as the matrix unit needs for the scores,
+// and in one stretch of code without dependences the two overlap.
 template <int D, int NT>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
@@ -816,23 +875,25 @@ struct many_t {
     static constexpr int DT = D / 16;
     static constexpr int WINDOW = 256, TPW = WINDOW / KT;
     struct shared_t {
-        deal_t  deal;
-        int     limit[ROWS];
-        int64_t entry[2][WINDOW];
-        int     page[WINDOW];
-        int     holes;     // some position has no page
-        int     flags[2];  // a tile's values were not all finite
-        half8_t k[NS][KT][CH], v[NS][KT][CH];
+        deal_t      deal;
+        int         limit[ROWS];
+        char const* kat[2][WINDOW];  // where the entries of a window's positions lie
+        char const* vat[2][WINDOW];
+        int         page[WINDOW];
+        int         least[WAVES];
+        int         holes;     // some position has no page
+        int         flags[2];  // a tile's values were not all finite
+        half8_t     k[NS][KT][CH], v[NS][KT][CH];
     };
 };
 
-template <int D, int NT>
+template <int D, int NT, bool PAD>
 __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kernel(attention_dev_t a)
 {
     typedef many_t<D, NT> M;
     typedef _Float16      T;
     constexpr int         ROWS = M::ROWS, KT = M::KT, CH = M::CH, DT = M::DT, NS = M::NS;
-    constexpr int         LPT = M::LPT;
+    constexpr int         LPT = M::LPT, ST = KT / 16;
     __shared__ typename M::shared_t sh;
     int const tid = int(threadIdx.x), lane = tid & 63;
     int const w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -841,6 +902,18 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     unit_of_block(a, unit, kvh);
     work_t wk;
     if (!deal<ROWS, 32>(a, sh.deal, sh.limit, unit, kvh, wk)) return;
+    int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
+    int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
+    int const first = lo / 32 * 32;
+
+    // this thread's position of window n, and its page number
+    auto position = [&](int n) { return first + n * M::WINDOW + tid; };
+    auto page_at = [&](int pos) {
+        return wk.table + (pos >= lo && pos < hi ? page_of(a, pos) : page_of(a, lo));
+    };
+    int page0 = -1;
+    if (lo < hi) page0 = *page_at(position(0));
+
     row_t row[NT];
     int   least = 0x7fffffff, most = -1;
 #pragma unroll
@@ -856,8 +929,6 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
     least = __builtin_amdgcn_readfirstlane(least);
     most = __builtin_amdgcn_readfirstlane(most);
-    int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
-    int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
 
     half8_t  q[NT][D / 32];
     float4_t o[NT][DT];
@@ -869,9 +940,10 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                              uint64_t(row[n].head) * uint64_t(a.d);
 #pragma unroll
         for (int i = 0; i != D / 32; ++i) {
-            int const e = i * 32 + g * 8;
-            q[n][i] = *reinterpret_cast<half8_t const*>(src + (e < a.d ? e : 0)) * T(a.q_sign);
-            if (e >= a.d) q[n][i] = half8_t{};
+            int const  e = i * 32 + g * 8;
+            bool const in = !PAD || e < a.d;
+            q[n][i] = *reinterpret_cast<half8_t const*>(src + (in ? e : 0)) * T(a.q_sign);
+            if (PAD && !in) q[n][i] = half8_t{};
         }
 #pragma unroll
         for (int t = 0; t != DT; ++t) o[n][t] = float4_t{0, 0, 0, 0};
@@ -880,116 +952,51 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
 
     if (lo < hi) {
-        T const* const kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
-        T const* const vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
-        int const      first = lo / 32 * 32;
-        int const      tiles = (hi - first + KT - 1) / KT;
+        char const* const kb = a.k + uint64_t(kvh) * a.head_stride * 2;
+        char const* const vb = a.v + uint64_t(kvh) * a.head_stride * 2;
+        char const* const zeros = reinterpret_cast<char const*>(attention_zeros);
+        int const         tiles = (hi - first + KT - 1) / KT;
 
-        // this thread's position of window n
-        auto position = [&](int n) { return first + n * M::WINDOW + tid; };
-        auto ask_page = [&](int n) {  // page numbers of window n, to LDS
-            int const pos = position(n);
-            load_to_lds_4(wk.table + (pos >= lo && pos < hi ? page_of(a, pos) : page_of(a, lo)),
-                          lds_address(&sh.page[w * 64]));
-        };
-        auto put_entry = [&](int n) {
+        auto put_entry = [&](int n, int page) {
             int const pos = position(n);
             int64_t   at = -1;
             if (pos >= lo && pos < hi) {
-                at = entry_of(a, sh.page[tid], pos - page_of(a, pos) * a.page_size);
+                at = entry_of(a, page, pos - page_of(a, pos) * a.page_size);
                 if (at < 0) sh.holes = 1;
             }
-            sh.entry[n & 1][tid] = at;
+            sh.kat[n & 1][tid] = at < 0 ? zeros : kb + at * 2;
+            sh.vat[n & 1][tid] = at < 0 ? zeros : vb + at * 2;
         };
         // this lane's row and chunk in a load instruction
         int const lrow = lane / CH, lpos = lane % CH;
         auto      load_tile = [&](int tile) {
-            int64_t const* const entry =
-                &sh.entry[tile / M::TPW & 1][tile % M::TPW * KT];
-            int const slot = tile % NS;
+            int const win = tile / M::TPW & 1, at = tile % M::TPW * KT, slot = tile % NS;
 #pragma unroll
             for (int i = 0; i != LPT; ++i) {
-                int const     r0 = (i * WAVES + w) * M::RPL;
-                int const     r = r0 + lrow;
-                int64_t const at = entry[r];
-                int const     kc = lpos ^ (r & 15 & (CH - 1));
-                int const     vc = lpos ^ ((2 * (r & 7)) & (CH - 1));
-                void const*   zeros = attention_zeros;
-                load_to_lds_16(at >= 0 && kc * 8 < a.d ? kb + at + kc * 8 : zeros,
-                                    lds_address(&sh.k[slot][r0][0]));
-                load_to_lds_16(at >= 0 && vc * 8 < a.d ? vb + at + vc * 8 : zeros,
-                                    lds_address(&sh.v[slot][r0][0]));
+                int const   r0 = (i * WAVES + w) * M::RPL;
+                int const   r = r0 + lrow;
+                int const   kc = lpos ^ (r & 15 & (CH - 1));
+                int const   vc = lpos ^ ((2 * (r & 7)) & (CH - 1));
+                char const* kp = sh.kat[win][at + r] + kc * 16;
+                char const* vp = sh.vat[win][at + r] + vc * 16;
+                if (PAD) {
+                    kp = kc * 8 < a.d ? kp : zeros;
+                    vp = vc * 8 < a.d ? vp : zeros;
+                }
+                load_to_lds_16(kp, lds_address(&sh.k[slot][r0][0]));
+                load_to_lds_16(vp, lds_address(&sh.v[slot][r0][0]));
             }
         };
-        // the least limit of the workgroup's rows decides where values have to be looked at
-        __syncthreads();  // limit[] is read above
-        if (tid == 0) {
-            sh.limit[0] = 0x7fffffff;
-            sh.holes = sh.flags[0] = sh.flags[1] = 0;
-        }
-        ask_page(0);
-        wait_loads<0>();
-        __syncthreads();
-        if (lane == 0) atomicMin(&sh.limit[0], least);
-        put_entry(0);
-        __syncthreads();
-        int const all_see = __builtin_amdgcn_readfirstlane(sh.limit[0]);
-        ask_page(1);
+        auto scores = [&](int slot, float4_t(&s)[NT][ST]) {
 #pragma unroll
-        for (int i = 0; i != NS - 1; ++i) {
-            // beyond the last tile too: the wait below counts instructions (their entries are -1)
-            load_tile(i);
-        }
-        for (int tile = 0; tile < tiles; ++tile) {
-            int const slot = tile % NS, base = first + tile * KT;
-            wait_loads<2 * LPT*(NS - 2)>();
-            __syncthreads();
-            bool const masked = base + KT - 1 > all_see;
-            int        careful = 0;
-            if (masked) {
-                // Zero times an infinity or NaN is no zero: where some row may not see a key of
-                // the tile, values that are not finite become zeros, and are added afterwards to
-                // the rows that see them.
-                bool bad = false;
-                for (int i = tid; i < KT * CH; i += THREADS) {
-                    half8_t& x = sh.v[slot][i / CH][i % CH];
-                    half8_t  y = x;
-                    bool     any = false;
+            for (int n = 0; n != NT; ++n) {
 #pragma unroll
-                    for (int e = 0; e != 8; ++e) {
-                        if (!(y[e] - y[e] == T(0))) {
-                            y[e] = T(0);
-                            any = true;
-                        }
-                    }
-                    if (any) {
-                        x = y;
-                        bad = true;
-                    }
-                }
-                if (tid == 0) sh.flags[(tile + 1) & 1] = 0;
-                if (bad) sh.flags[tile & 1] = 1;
-                __syncthreads();
-                careful = __builtin_amdgcn_readfirstlane(sh.flags[tile & 1]);
+                for (int t = 0; t != ST; ++t) s[n][t] = float4_t{0, 0, 0, 0};
             }
-            {
-                // tile + NS - 1 goes where the last one was; windows are prepared on the way
-                int const j = tile + NS - 1;
-                load_tile(j);
-                int const n = j / M::TPW, at = j % M::TPW;
-                if (at == M::TPW - 2) put_entry(n + 1);
-                if (at == M::TPW - 1) ask_page(n + 2);
-            }
-            if (base > most) continue;
-            bool const holes = sh.holes != 0;
-            bool const edge = holes || base < lo || base + KT > hi || base + KT - 1 > least;
-            float4_t   s[NT][KT / 16];
 #pragma unroll
-            for (int t = 0; t != KT / 16; ++t) {
+            for (int i = 0; i != D / 32; ++i) {
 #pragma unroll
-                for (int n = 0; n != NT; ++n) s[n][t] = float4_t{0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i != D / 32; ++i) {
+                for (int t = 0; t != ST; ++t) {
                     half8_t const kf = sh.k[slot][16 * t + c][(4 * i + g) ^ (c & (CH - 1))];
 #pragma unroll
                     for (int n = 0; n != NT; ++n) {
@@ -998,36 +1005,113 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     }
                 }
             }
-            if (edge) {
-                int64_t const* const entry = &sh.entry[tile / M::TPW & 1][tile % M::TPW * KT];
+        };
+        // scores that a row may not see
+        auto mask = [&](int tile, float4_t(&s)[NT][ST]) {
+            int const base = first + tile * KT;
+            if (!(sh.holes != 0 || base < lo || base + KT > hi || base + KT - 1 > least)) return;
+            char const* const* const at = &sh.kat[tile / M::TPW & 1][tile % M::TPW * KT];
 #pragma unroll
-                for (int t = 0; t != KT / 16; ++t) {
+            for (int t = 0; t != ST; ++t) {
 #pragma unroll
-                    for (int r = 0; r != 4; ++r) {
-                        int const  key = 16 * t + 4 * g + r;
-                        bool const none = entry[key] < 0;  // not among the positions, or no page
+                for (int r = 0; r != 4; ++r) {
+                    int const  key = 16 * t + 4 * g + r;
+                    bool const none = at[key] == zeros;  // not among the positions, or no page
 #pragma unroll
-                        for (int n = 0; n != NT; ++n) {
-                            if (none || base + key > row[n].limit) s[n][t][r] = NEG_INF;
-                        }
+                    for (int n = 0; n != NT; ++n) {
+                        if (none || base + key > row[n].limit) s[n][t][r] = NEG_INF;
                     }
                 }
             }
-            half8_t p[NT][KT / 32];
+        };
+        auto top_of = [&](float4_t const(&s)[ST]) {
+            float top = NEG_INF;
+#pragma unroll
+            for (int t = 0; t != ST; ++t) {
+#pragma unroll
+                for (int r = 0; r != 4; ++r) top = fmaxf(top, s[t][r]);
+            }
+            return column_max(top) * a.scale;
+        };
+
+        if (tid == 0) sh.holes = sh.flags[0] = sh.flags[1] = 0;
+        if (lane == 0) sh.least[w] = least;
+        __syncthreads();
+        put_entry(0, page0);
+        __syncthreads();
+        // the least limit of the workgroup's rows decides where values have to be looked at
+        int const all_see = __builtin_amdgcn_readfirstlane(
+            min(min(sh.least[0], sh.least[1]), min(sh.least[2], sh.least[3])));
+        // Zero times an infinity or NaN is no zero: where some row may not see a key of the tile,
+        // values that are not finite become zeros, and are added afterwards to the rows that see
+        // them.  True: there were some.
+        auto clean = [&](int tile) {
+            if (first + tile * KT + KT - 1 <= all_see) return 0;
+            bool bad = false;
+            for (int i = tid; i < KT * CH; i += THREADS) {
+                half8_t& x = sh.v[tile % NS][i / CH][i % CH];
+                half8_t  y = x;
+                bool     any = false;
+#pragma unroll
+                for (int e = 0; e != 8; ++e) {
+                    if (!(y[e] - y[e] == T(0))) {
+                        y[e] = T(0);
+                        any = true;
+                    }
+                }
+                if (any) {
+                    x = y;
+                    bad = true;
+                }
+            }
+            if (tid == 0) sh.flags[(tile + 1) & 1] = 0;
+            if (bad) sh.flags[tile & 1] = 1;
+            __syncthreads();
+            return __builtin_amdgcn_readfirstlane(sh.flags[tile & 1]);
+        };
+        {
+            int const pos = position(1);
+            load_to_lds_4(page_at(pos), lds_address(&sh.page[w * 64]));
+        }
+        // beyond the last tile too: the waits count instructions (the entries are zeros)
+#pragma unroll
+        for (int i = 0; i != NS - 1; ++i) load_tile(i);
+        wait_loads<2 * LPT*(NS - 2)>();
+        __syncthreads();
+        int      careful = clean(0);
+        float4_t s[NT][ST];
+        scores(0, s);
+        mask(0, s);
+#pragma unroll
+        for (int n = 0; n != NT; ++n) raise<DT>(top_of(s[n]), m[n], l[n], o[n]);
+
+        for (int tile = 0; tile < tiles; ++tile) {
+            int const base = first + tile * KT;
+            wait_loads<2 * LPT*(NS - 3)>();
+            __syncthreads();
+            int const careful_next = clean(tile + 1);
+            {
+                // tile + NS - 1 goes where the last one was; windows are prepared on the way
+                int const j = tile + NS - 1;
+                load_tile(j);
+                int const n = j / M::TPW, at = j % M::TPW;
+                if (at == M::TPW - 2) put_entry(n + 1, sh.page[tid]);
+                if (at == M::TPW - 1) {
+                    load_to_lds_4(page_at(position(n + 2)), lds_address(&sh.page[w * 64]));
+                }
+            }
+            int const now = careful;
+            careful = careful_next;
+            if (base > most) continue;
+            half8_t  p[NT][KT / 32];
+            float4_t next[NT][ST];
+            scores((tile + 1) % NS, next);
 #pragma unroll
             for (int n = 0; n != NT; ++n) {
-                float top = NEG_INF;
-#pragma unroll
-                for (int t = 0; t != KT / 16; ++t) {
-#pragma unroll
-                    for (int r = 0; r != 4; ++r) top = fmaxf(top, s[n][t][r]);
-                }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                float const ref = raise<DT>(top * a.scale, m[n], l[n], o[n]);
+                float const ref = m[n] == NEG_INF ? 0.0f : m[n];
                 float       sum = 0;
 #pragma unroll
-                for (int t = 0; t != KT / 16; ++t) {
+                for (int t = 0; t != ST; ++t) {
 #pragma unroll
                     for (int r = 0; r != 4; ++r) {
                         float const e = exp2_fast(s[n][t][r] * a.scale - ref);
@@ -1037,6 +1121,10 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                 }
                 l[n] += sum;
             }
+            mask(tile + 1, next);
+            float top[NT];
+#pragma unroll
+            for (int n = 0; n != NT; ++n) top[n] = top_of(next[n]);
             // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of its
             // own element
             typedef short tr_t __attribute__((ext_vector_type(4)));
@@ -1052,7 +1140,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     for (int half = 0; half != 2; ++half) {
                         int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
                         int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
-                        char* at = reinterpret_cast<char*>(&sh.v[slot][r][chunk]) + (c & 1) * 8;
+                        char*     at = reinterpret_cast<char*>(&sh.v[tile % NS][r][chunk]) +
+                                   (c & 1) * 8;
                         vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) tr_t*)(at));
                     }
@@ -1063,17 +1152,18 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     }
                 }
             }
-            if (careful) {
+            if (now) {
+#pragma nounroll
                 for (int i = 0; i != KT; ++i) {
-                    int64_t const at = sh.entry[tile / M::TPW & 1][tile % M::TPW * KT + i];
-                    if (at < 0) continue;
+                    char const* const at = sh.vat[tile / M::TPW & 1][tile % M::TPW * KT + i];
+                    if (at == zeros) continue;
 #pragma unroll
                     for (int t = 0; t != DT; ++t) {
 #pragma unroll
                         for (int r = 0; r != 4; ++r) {
                             int const e = 16 * t + 4 * g + r;
-                            if (e >= a.d) continue;
-                            float const x = float(vb[at + e]);
+                            if (PAD && e >= a.d) continue;
+                            float const x = float(reinterpret_cast<T const*>(at)[e]);
                             if (x - x == 0.0f) continue;
 #pragma unroll
                             for (int n = 0; n != NT; ++n) {
@@ -1083,14 +1173,19 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     }
                 }
             }
+#pragma unroll
+            for (int n = 0; n != NT; ++n) {
+                raise<DT>(top[n], m[n], l[n], o[n]);
+#pragma unroll
+                for (int t = 0; t != ST; ++t) s[n][t] = next[n][t];
+            }
         }
         // nothing may still be on its way to LDS when the workgroup ends
         wait_loads<0>();
     }
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
-        l[n] += __shfl_xor(l[n], 16);
-        l[n] += __shfl_xor(l[n], 32);
+        l[n] = column_sum(l[n]);
         if (row[n].token < 0) continue;
         // O^T: elements 16 t + 4 g + r of this lane's row
         if (wk.direct) {
@@ -1210,12 +1305,20 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
     if constexpr (sizeof(T) == 2) {
         if constexpr (D <= 128) {
             if (rows == many_t<D, 2>::ROWS) {
-                attention_many_kernel<D, 2><<<grid, THREADS, 0, stream>>>(a);
+                if (a.d == D) {
+                    attention_many_kernel<D, 2, false><<<grid, THREADS, 0, stream>>>(a);
+                } else {
+                    attention_many_kernel<D, 2, true><<<grid, THREADS, 0, stream>>>(a);
+                }
                 return;
             }
         }
         if (rows == many_t<D, 1>::ROWS) {
-            attention_many_kernel<D, 1><<<grid, THREADS, 0, stream>>>(a);
+            if (a.d == D) {
+                attention_many_kernel<D, 1, false><<<grid, THREADS, 0, stream>>>(a);
+            } else {
+                attention_many_kernel<D, 1, true><<<grid, THREADS, 0, stream>>>(a);
+            }
             return;
         }
     }
