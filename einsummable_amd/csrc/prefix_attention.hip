@@ -1161,13 +1161,13 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     for (int t = 0; t != DT; ++t) {
 #pragma unroll
                         for (int r = 0; r != 4; ++r) {
-                            int const e = 16 * t + 4 * g + r;
-                            if (PAD && e >= a.d) continue;
-                            float const x = float(reinterpret_cast<T const*>(at)[e]);
-                            if (x - x == 0.0f) continue;
+                            int const   e = 16 * t + 4 * g + r;
+                            float const x =
+                                float(reinterpret_cast<T const*>(at)[!PAD || e < a.d ? e : 0]);
+                            bool const add = !(x - x == 0.0f) && (!PAD || e < a.d);
 #pragma unroll
                             for (int n = 0; n != NT; ++n) {
-                                if (base + i <= row[n].limit) o[n][t][r] += x;
+                                o[n][t][r] += add && base + i <= row[n].limit ? x : 0.0f;
                             }
                         }
                     }
@@ -1214,24 +1214,26 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
 }
 
-// One wavefront per row: the maxima and sums of its cuts decide their weights, then the cuts'
+// Sixteen lanes per row: the references and sums of its cuts decide their weights, then the cuts'
 // O are added in order.
 template <typename T, int D>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t a)
 {
-    int const lane = int(threadIdx.x) & 63, w = int(threadIdx.x) >> 6;
-    int const heads = a.h_kv * a.group;
-    int const id = int(blockIdx.x) * WAVES + w;
-    int const token = id / heads, head = id - token * heads;
+    constexpr int LANES = 16, PER = D / LANES;
+    int const     lane = int(threadIdx.x) % LANES;
+    int const     heads = a.h_kv * a.group;
+    int const     id = int(blockIdx.x) * (THREADS / LANES) + int(threadIdx.x) / LANES;
+    int const     token = id / heads, head = id - token * heads;
     if (token >= a.n_tokens) return;
-    if (token < a.offsets[0] || token >= a.offsets[a.n_seqs]) return;
     int const* const meta = a.part_meta + 4 * token;
-    int const        splits = min(meta[1], a.items), b = meta[2];
+    int const        from = meta[0], said = meta[1], b = meta[2];
+    if (token < a.offsets[0] || token >= a.offsets[a.n_seqs]) return;
+    int const splits = min(said, a.items);
     if (splits <= 0) return;
     int const kvh = head / a.group, hg = head - kvh * a.group;
     int const prow = token * a.group + hg, srow = (token - b) * a.group + hg;
-    int const pslot = prow / a.prefix_rows;
-    int const sslot = meta[0] + srow / a.own_rows * splits;
+    int const pslot = a.prefix_splits ? prow / a.prefix_rows : 0;
+    int const sslot = from + srow / a.own_rows * splits;
     int const parts = a.prefix_splits + splits;
     auto      place = [&](int i) -> int64_t {
         if (i < a.prefix_splits) {
@@ -1244,14 +1246,15 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
                max(srow, 0) % a.own_rows;
     };
     float top = NEG_INF;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, a.part_ml[place(i) * 2]);
+    for (int i = lane; i < parts; i += LANES) top = fmaxf(top, a.part_ml[place(i) * 2]);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    constexpr int PER = D / 64;
-    float         y[PER], sum = 0;
+    for (int o = LANES / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    float4_t y[PER / 4];
+    float    sum = 0;
 #pragma unroll
-    for (int e = 0; e != PER; ++e) y[e] = 0;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
+    for (int e = 0; e != PER / 4; ++e) y[e] = float4_t{0, 0, 0, 0};
+    int const group0 = int(threadIdx.x) & 63 & ~(LANES - 1);
+    for (int i0 = 0; i0 < parts; i0 += LANES) {
         // lane i: the place and the weight of cut i0 + i; none without keys for this row
         bool const    in = i0 + lane < parts;
         int64_t const at = in ? place(i0 + lane) : 0;
@@ -1259,35 +1262,48 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
         float const   li = in ? a.part_ml[at * 2 + 1] : 0.0f;
         float const   f = mi == NEG_INF ? 0.0f : exp2_fast(mi - top);
         sum += mi == NEG_INF ? 0.0f : li * f;
-        constexpr int U = 8;  // cuts in flight
-        int const     n = min(parts - i0, 64);
+        constexpr int U = 4;  // cuts in flight
+        int const     n = min(parts - i0, LANES);
         for (int i = 0; i < n; i += U) {
-            float x[U][PER], fi[U];
+            float4_t x[U][PER / 4];
+            float    fi[U];
 #pragma unroll
             for (int u = 0; u != U; ++u) {
-                int const     from = min(i + u, n - 1);
-                int64_t const p = __shfl(at, from);
-                fi[u] = i + u < n ? __shfl(f, from) : 0.0f;
+                int const     which = group0 + min(i + u, n - 1);
+                int64_t const p = __shfl(at, which);
+                float const   fu = __shfl(f, which);
+                fi[u] = i + u < n ? fu : 0.0f;
+                // a cut without weight may hold anything
+                float4_t const* const src =
+                    reinterpret_cast<float4_t const*>(a.part_o + p * D + lane * PER);
 #pragma unroll
-                for (int e = 0; e != PER; ++e) {
-                    x[u][e] = fi[u] != 0.0f ? a.part_o[p * D + lane * PER + e] : 0.0f;
+                for (int e = 0; e != PER / 4; ++e) {
+                    x[u][e] = fi[u] != 0.0f ? src[e] : float4_t{0, 0, 0, 0};
                 }
             }
 #pragma unroll
             for (int u = 0; u != U; ++u) {
 #pragma unroll
-                for (int e = 0; e != PER; ++e) y[e] += x[u][e] * fi[u];
+                for (int e = 0; e != PER / 4; ++e) y[e] += x[u][e] * fi[u];
             }
         }
     }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor(sum, o);
     T* const    dst = reinterpret_cast<T*>(a.out) + uint64_t(token) * a.out_stride +
                    uint64_t(head) * uint64_t(a.d) + lane * PER;
     float const inv = top == NEG_INF ? 0.0f : 1.0f / sum;
+    // in vectors of at most 16 bytes; d is a multiple of 8
+    constexpr int V = PER < 16 / int(sizeof(T)) ? PER : 16 / int(sizeof(T));
+    typedef T     vec_t __attribute__((ext_vector_type(V)));
 #pragma unroll
-    for (int e = 0; e != PER; ++e) {
-        if (lane * PER + e < a.d) dst[e] = T(top == NEG_INF ? 0.0f : y[e] * inv);
+    for (int e = 0; e != PER; e += V) {
+        vec_t z;
+#pragma unroll
+        for (int i = 0; i != V; ++i) {
+            z[i] = T(top == NEG_INF ? 0.0f : y[(e + i) / 4][(e + i) % 4] * inv);
+        }
+        if (lane * PER + e < a.d) *reinterpret_cast<vec_t*>(dst + e) = z;
     }
 }
 
@@ -1340,7 +1356,7 @@ void launch_dim(attention_dev_t const& a, hipStream_t stream)
     }
     if (a.prefix_splits != 0 || a.split_target != 0) {
         uint64_t const rows = uint64_t(a.n_tokens) * a.h_kv * a.group;
-        attention_join_kernel<T, D><<<uint32_t((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(a);
+        attention_join_kernel<T, D><<<uint32_t((rows + 15) / 16), THREADS, 0, stream>>>(a);
     }
 }
 
