@@ -35,6 +35,7 @@
 #include "serving_device.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace es
 {
@@ -595,22 +596,23 @@ struct core_t<float, D> {
     }
 };
 
-// Takes the largest score of a step into a row's reference m (what exponents are taken relative
-// to) and returns the reference to use, 0 while nothing was seen.  The reference need not be the
-// maximum: it is raised, and what was summed so far scaled down, only where a score passes it by
-// 2^8, which leaves p below 2^8 and f16's relative precision as it is.
+// Takes the scores of a step into a row's reference m, what exponents are taken relative to
+// (`top`: the largest of this lane's).  The reference need not be the maximum: it is raised, and
+// what was summed so far scaled down, only where a score passes it by 2^8, which leaves p below
+// 2^8 and f16's relative precision as it is; so the lanes of a column have to agree on their
+// maximum only then.  `ref` is m, or 0 while nothing was seen.
 template <int N>
-__device__ inline float raise(float top, float& m, float& l, float4_t* o)
+__device__ inline void raise(float top, float& m, float& ref, float& l, float4_t* o)
 {
     if (__any(top > m + 8.0f)) {
-        float const mn = fmaxf(m, top);
-        float const fade = exp2_fast(m - (mn == NEG_INF ? 0.0f : mn));
+        float const mn = fmaxf(m, column_max(top));
+        ref = mn == NEG_INF ? 0.0f : mn;
+        float const fade = exp2_fast(m - ref);
         l *= fade;
 #pragma unroll
         for (int t = 0; t != N; ++t) o[t] *= fade;
         m = mn;
     }
-    return m == NEG_INF ? 0.0f : m;
 }
 
 // ------------------------------------------------------------------------------ few rows
@@ -659,7 +661,8 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             page = wk.table[pi];
         }
     };
-    int base = (lo / KS + w) * KS;
+    int   base = (lo / KS + w) * KS;
+    float ref = 0;
     look_up(base);
     for (; base < hi; base += WAVES * KS) {
         int64_t const at = entry_of(a, page, prow);
@@ -691,9 +694,8 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             s[j] = masked >> j & 1 ? NEG_INF : s[j];
             top = fmaxf(top, s[j]);
         }
-        top = column_max(top);
-        float const ref = raise<DV>(top * a.scale, m, l, o);
-        float       sum = 0;
+        raise<DV>(top * a.scale, m, ref, l, o);
+        float sum = 0;
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
             s[j] = exp2_fast(s[j] * a.scale - ref);
@@ -864,11 +866,12 @@ __device__ __forceinline__ uint32_t lds_address(void const* p)
 // The scores of tile i + 1 are computed in the iteration that turns those of tile i into weights:
 // the exponentials take the vector unit about as long as the matrix unit needs for the scores,
 // and in one stretch of code without dependences the two overlap.
+// The sum of a row's weights is one more row of O^T, with ones for V^T.
 template <int D, int NT>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
     static constexpr int KT = 32;
-    static constexpr int NS = D == 256 ? 3 : 4;
+    static constexpr int NS = 4;
     static constexpr int CH = D / 8;             // chunks per row
     static constexpr int RPL = 64 / CH;          // rows per load instruction
     static constexpr int LPT = KT / RPL / WAVES; // load instructions per wavefront and tile, of K
@@ -881,8 +884,8 @@ struct many_t {
         char const* vat[2][WINDOW];
         int         page[WINDOW];
         int         least[WAVES];
-        int         holes;     // some position has no page
-        int         flags[2];  // a tile's values were not all finite
+        int         holes;  // some position has no page
+        int         bad;    // some value was not finite
         half8_t     k[NS][KT][CH], v[NS][KT][CH];
     };
 };
@@ -931,8 +934,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     most = __builtin_amdgcn_readfirstlane(most);
 
     half8_t  q[NT][D / 32];
-    float4_t o[NT][DT];
-    float    m[NT], l[NT];
+    float4_t o[NT][DT + 1];  // [DT]: the sum of the weights, four times
+    float    m[NT], ref[NT];
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
         T const* const src = reinterpret_cast<T const*>(a.q) +
@@ -946,9 +949,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             if (PAD && !in) q[n][i] = half8_t{};
         }
 #pragma unroll
-        for (int t = 0; t != DT; ++t) o[n][t] = float4_t{0, 0, 0, 0};
+        for (int t = 0; t != DT + 1; ++t) o[n][t] = float4_t{0, 0, 0, 0};
         m[n] = NEG_INF;
-        l[n] = 0;
+        ref[n] = 0;
     }
 
     if (lo < hi) {
@@ -967,24 +970,34 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             sh.kat[n & 1][tid] = at < 0 ? zeros : kb + at * 2;
             sh.vat[n & 1][tid] = at < 0 ? zeros : vb + at * 2;
         };
-        // this lane's row and chunk in a load instruction
-        int const lrow = lane / CH, lpos = lane % CH;
-        auto      load_tile = [&](int tile) {
-            int const win = tile / M::TPW & 1, at = tile % M::TPW * KT, slot = tile % NS;
+        // this lane's row and chunk in a load instruction; the addresses of a tile are read from
+        // the window a tile before its loads go out
+        int const   lrow = lane / CH, lpos = lane % CH;
+        char const *kp[LPT], *vp[LPT];
+        auto        aim = [&](int tile) {
+            int const win = tile / M::TPW & 1, at = tile % M::TPW * KT;
 #pragma unroll
             for (int i = 0; i != LPT; ++i) {
-                int const   r0 = (i * WAVES + w) * M::RPL;
-                int const   r = r0 + lrow;
-                int const   kc = lpos ^ (r & 15 & (CH - 1));
-                int const   vc = lpos ^ ((2 * (r & 7)) & (CH - 1));
-                char const* kp = sh.kat[win][at + r] + kc * 16;
-                char const* vp = sh.vat[win][at + r] + vc * 16;
+                int const r = (i * WAVES + w) * M::RPL + lrow;
+                int const kc = lpos ^ (r & 15 & (CH - 1));
+                int const vc = lpos ^ ((2 * (r & 7)) & (CH - 1));
+                kp[i] = sh.kat[win][at + r] + kc * 16;
+                vp[i] = sh.vat[win][at + r] + vc * 16;
                 if (PAD) {
-                    kp = kc * 8 < a.d ? kp : zeros;
-                    vp = vc * 8 < a.d ? vp : zeros;
+                    kp[i] = kc * 8 < a.d ? kp[i] : zeros;
+                    vp[i] = vc * 8 < a.d ? vp[i] : zeros;
                 }
-                load_to_lds_16(kp, lds_address(&sh.k[slot][r0][0]));
-                load_to_lds_16(vp, lds_address(&sh.v[slot][r0][0]));
+            }
+        };
+        uint32_t const lds_k = lds_address(&sh.k[0][w * M::RPL][0]);
+        uint32_t const lds_v = lds_address(&sh.v[0][w * M::RPL][0]);
+        auto           load_tile = [&](int tile) {
+            uint32_t const slot = uint32_t(tile % NS) * uint32_t(KT * D * 2);
+#pragma unroll
+            for (int i = 0; i != LPT; ++i) {
+                uint32_t const at = slot + uint32_t(i * WAVES * M::RPL * D * 2);
+                load_to_lds_16(kp[i], lds_k + at);
+                load_to_lds_16(vp[i], lds_v + at);
             }
         };
         auto scores = [&](int slot, float4_t(&s)[NT][ST]) {
@@ -1006,10 +1019,13 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                 }
             }
         };
-        // scores that a row may not see
+        // whether there are positions in a tile that some row may not see
+        auto edge = [&](int tile) {
+            int const base = first + tile * KT;
+            return sh.holes != 0 || base < lo || base + KT > hi || base + KT - 1 > least;
+        };
         auto mask = [&](int tile, float4_t(&s)[NT][ST]) {
             int const base = first + tile * KT;
-            if (!(sh.holes != 0 || base < lo || base + KT > hi || base + KT - 1 > least)) return;
             char const* const* const at = &sh.kat[tile / M::TPW & 1][tile % M::TPW * KT];
 #pragma unroll
             for (int t = 0; t != ST; ++t) {
@@ -1024,6 +1040,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                 }
             }
         };
+        // the largest of this lane's scores of a row
         auto top_of = [&](float4_t const(&s)[ST]) {
             float top = NEG_INF;
 #pragma unroll
@@ -1031,10 +1048,17 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
 #pragma unroll
                 for (int r = 0; r != 4; ++r) top = fmaxf(top, s[t][r]);
             }
-            return column_max(top) * a.scale;
+            return top * a.scale;
+        };
+        auto raise_all = [&](float4_t const(&s)[NT][ST]) {
+#pragma unroll
+            for (int n = 0; n != NT; ++n) {
+                float none = 0;
+                raise<DT + 1>(top_of(s[n]), m[n], ref[n], none, o[n]);
+            }
         };
 
-        if (tid == 0) sh.holes = sh.flags[0] = sh.flags[1] = 0;
+        if (tid == 0) sh.holes = sh.bad = 0;
         if (lane == 0) sh.least[w] = least;
         __syncthreads();
         put_entry(0, page0);
@@ -1043,11 +1067,10 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         int const all_see = __builtin_amdgcn_readfirstlane(
             min(min(sh.least[0], sh.least[1]), min(sh.least[2], sh.least[3])));
         // Zero times an infinity or NaN is no zero: where some row may not see a key of the tile,
-        // values that are not finite become zeros, and are added afterwards to the rows that see
-        // them.  True: there were some.
+        // values that are not finite become zeros, and are added in the end to the rows that see
+        // them.
         auto clean = [&](int tile) {
-            if (first + tile * KT + KT - 1 <= all_see) return 0;
-            bool bad = false;
+            if (first + tile * KT + KT - 1 <= all_see) return;
             for (int i = tid; i < KT * CH; i += THREADS) {
                 half8_t& x = sh.v[tile % NS][i / CH][i % CH];
                 half8_t  y = x;
@@ -1061,70 +1084,63 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                 }
                 if (any) {
                     x = y;
-                    bad = true;
+                    sh.bad = 1;
                 }
             }
-            if (tid == 0) sh.flags[(tile + 1) & 1] = 0;
-            if (bad) sh.flags[tile & 1] = 1;
             __syncthreads();
-            return __builtin_amdgcn_readfirstlane(sh.flags[tile & 1]);
         };
-        {
-            int const pos = position(1);
-            load_to_lds_4(page_at(pos), lds_address(&sh.page[w * 64]));
-        }
+        load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
         // beyond the last tile too: the waits count instructions (the entries are zeros)
 #pragma unroll
-        for (int i = 0; i != NS - 1; ++i) load_tile(i);
+        for (int i = 0; i != NS - 1; ++i) {
+            aim(i);
+            load_tile(i);
+        }
+        aim(NS - 1);
         wait_loads<2 * LPT*(NS - 2)>();
         __syncthreads();
-        int      careful = clean(0);
-        float4_t s[NT][ST];
-        scores(0, s);
-        mask(0, s);
-#pragma unroll
-        for (int n = 0; n != NT; ++n) raise<DT>(top_of(s[n]), m[n], l[n], o[n]);
+        clean(0);
+        float4_t s[2][NT][ST];
+        scores(0, s[0]);
+        if (edge(0)) mask(0, s[0]);
+        raise_all(s[0]);
 
-        for (int tile = 0; tile < tiles; ++tile) {
-            int const base = first + tile * KT;
+        half8_t ones;
+#pragma unroll
+        for (int e = 0; e != 8; ++e) ones[e] = T(1);
+        // weights of a tile, scores of the next one, O.  SLOT, the tile's modulo NS, is known to
+        // the compiler: places in LDS are then offsets of the instructions.
+        auto step = [&](int tile, auto slot_) {
+            constexpr int SLOT = decltype(slot_)::value;
+            float4_t(&now)[NT][ST] = s[SLOT & 1];
+            float4_t(&next)[NT][ST] = s[(SLOT + 1) & 1];
             wait_loads<2 * LPT*(NS - 3)>();
             __syncthreads();
-            int const careful_next = clean(tile + 1);
-            {
-                // tile + NS - 1 goes where the last one was; windows are prepared on the way
-                int const j = tile + NS - 1;
-                load_tile(j);
-                int const n = j / M::TPW, at = j % M::TPW;
-                if (at == M::TPW - 2) put_entry(n + 1, sh.page[tid]);
-                if (at == M::TPW - 1) {
-                    load_to_lds_4(page_at(position(n + 2)), lds_address(&sh.page[w * 64]));
-                }
+            // tile + NS - 1 goes where the last one was; windows are prepared on the way
+            int const j = tile + NS - 1;
+            load_tile(j);
+            clean(tile + 1);
+            int const n = j / M::TPW, at = j % M::TPW;
+            if (at == M::TPW - 3) put_entry(n + 1, sh.page[tid]);
+            if (at == M::TPW - 1) {
+                load_to_lds_4(page_at(position(n + 2)), lds_address(&sh.page[w * 64]));
             }
-            int const now = careful;
-            careful = careful_next;
-            if (base > most) continue;
-            half8_t  p[NT][KT / 32];
-            float4_t next[NT][ST];
-            scores((tile + 1) % NS, next);
+            aim(j + 1);
+            if (first + tile * KT > most) return;
+            scores((SLOT + 1) % NS, next);
+            half8_t p[NT][KT / 32];
 #pragma unroll
             for (int n = 0; n != NT; ++n) {
-                float const ref = m[n] == NEG_INF ? 0.0f : m[n];
-                float       sum = 0;
 #pragma unroll
                 for (int t = 0; t != ST; ++t) {
 #pragma unroll
                     for (int r = 0; r != 4; ++r) {
-                        float const e = exp2_fast(s[n][t][r] * a.scale - ref);
-                        sum += e;
-                        p[n][t / 2][4 * (t & 1) + r] = T(e);
+                        p[n][t / 2][4 * (t & 1) + r] =
+                            T(exp2_fast(now[n][t][r] * a.scale - ref[n]));
                     }
                 }
-                l[n] += sum;
             }
-            mask(tile + 1, next);
-            float top[NT];
-#pragma unroll
-            for (int n = 0; n != NT; ++n) top[n] = top_of(next[n]);
+            if (edge(tile + 1)) mask(tile + 1, next);
             // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of its
             // own element
             typedef short tr_t __attribute__((ext_vector_type(4)));
@@ -1140,8 +1156,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     for (int half = 0; half != 2; ++half) {
                         int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
                         int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
-                        char*     at = reinterpret_cast<char*>(&sh.v[tile % NS][r][chunk]) +
-                                   (c & 1) * 8;
+                        char*     at = reinterpret_cast<char*>(&sh.v[SLOT][r][chunk]) + (c & 1) * 8;
                         vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) tr_t*)(at));
                     }
@@ -1152,32 +1167,42 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     }
                 }
             }
-            if (now) {
-#pragma nounroll
-                for (int i = 0; i != KT; ++i) {
-                    char const* const at = sh.vat[tile / M::TPW & 1][tile % M::TPW * KT + i];
-                    if (at == zeros) continue;
 #pragma unroll
-                    for (int t = 0; t != DT; ++t) {
+            for (int n = 0; n != NT; ++n) {
 #pragma unroll
-                        for (int r = 0; r != 4; ++r) {
-                            int const   e = 16 * t + 4 * g + r;
-                            float const x =
-                                float(reinterpret_cast<T const*>(at)[!PAD || e < a.d ? e : 0]);
-                            bool const add = !(x - x == 0.0f) && (!PAD || e < a.d);
+                for (int ks = 0; ks != KT / 32; ++ks) {
+                    o[n][DT] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[n][ks], o[n][DT], 0, 0, 0);
+                }
+            }
+            raise_all(next);
+        };
+        for (int tile = 0; tile < tiles; tile += NS) {
+            step(tile, std::integral_constant<int, 0>());
+            if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>());
+            if (tile + 2 < tiles) step(tile + 2, std::integral_constant<int, 2>());
+            if (tile + 3 < tiles) step(tile + 3, std::integral_constant<int, 3>());
+        }
+        __syncthreads();
+        if (sh.bad) {
+            for (int pos = max(lo, (all_see - first + 1) / KT * KT + first); pos < hi; ++pos) {
+                int const     pi = page_of(a, pos);
+                int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
+                if (at < 0) continue;
+                T const* const value = reinterpret_cast<T const*>(vb + at * 2);
 #pragma unroll
-                            for (int n = 0; n != NT; ++n) {
-                                o[n][t][r] += add && base + i <= row[n].limit ? x : 0.0f;
-                            }
+                for (int t = 0; t != DT; ++t) {
+#pragma unroll
+                    for (int r = 0; r != 4; ++r) {
+                        int const   e = 16 * t + 4 * g + r;
+                        float const x = float(value[!PAD || e < a.d ? e : 0]);
+                        bool const  add = !(x - x == 0.0f) && (!PAD || e < a.d);
+#pragma unroll
+                        for (int n = 0; n != NT; ++n) {
+                            o[n][t][r] += add && pos <= row[n].limit ? x : 0.0f;
                         }
                     }
                 }
-            }
-#pragma unroll
-            for (int n = 0; n != NT; ++n) {
-                raise<DT>(top[n], m[n], l[n], o[n]);
-#pragma unroll
-                for (int t = 0; t != ST; ++t) s[n][t] = next[n][t];
             }
         }
         // nothing may still be on its way to LDS when the workgroup ends
@@ -1185,13 +1210,12 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
-        l[n] = column_sum(l[n]);
         if (row[n].token < 0) continue;
         // O^T: elements 16 t + 4 g + r of this lane's row
         if (wk.direct) {
             T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(row[n].token) * a.out_stride +
                            uint64_t(row[n].head) * uint64_t(a.d);
-            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / l[n];
+            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / o[n][DT][0];
 #pragma unroll
             for (int t = 0; t != DT; ++t) {
                 int const e = 16 * t + 4 * g;
@@ -1208,7 +1232,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             }
             if (g == 0) {
                 a.part_ml[at * 2] = m[n];
-                a.part_ml[at * 2 + 1] = l[n];
+                a.part_ml[at * 2 + 1] = o[n][DT][0];
             }
         }
     }
