@@ -2,7 +2,7 @@
 // that all sequences share read once for many rows.
 //
 // A row is a query: token i, head h.  The rows that read one key head (h' = h / G) are dealt
-// with in tiles of 16, the keys in steps of KS (32 in f16, 16 in f32), one pass with a running
+// with in tiles of 16, the keys in steps of 16 or 32, one pass with a running
 // maximum m and sum l per row:
 //
 //   S^T = K Q^T             rows are keys, columns are the tile's queries
@@ -11,11 +11,11 @@
 //
 // Both products are taken transposed because of what the matrix instructions' registers hold:
 // lane (g, c), g = lane / 16, c = lane % 16, gets column c of a result, so a query's maximum,
-// sum and scaling live in the lanes of its own column, and the four (f32) or eight (f16) scores
-// a lane gets are exactly the slice of P^T it has to supply to the second product -- for the
-// keys 16 t + 4 g + r, which is then the order the lane reads the rows of V in (a sum over keys
-// has no preferred order).  Neither K nor V nor P passes through LDS.  A lane's rows of V are
-// consecutive elements of 4 or 8 keys; in f16 they are transposed in registers (v_perm_b32).
+// sum and scaling live in the lanes of its own column, and the four scores a lane gets of
+// sixteen keys are exactly the slice of P^T it has to supply to the second product -- for the
+// keys 4 g + r, which is then the order the lane reads the rows of V in (a sum over keys has no
+// preferred order).  Neither K nor V nor P passes through LDS.  A lane's rows of V are
+// consecutive elements of four keys; in f16 they are transposed in registers (v_perm_b32).
 //
 // Two kernels.  attention_few_kernel, for decoding: tiles of 16 rows; the four wavefronts of a
 // workgroup take the steps of its keys in turn, straight from global memory into registers (K
@@ -348,56 +348,57 @@ __device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit,
 template <typename T, int D>
 struct core_t;
 
-// ---- f16: steps of 32 keys, v_mfma_f32_16x16x32_f16
+// ---- f16: steps of 16 keys, v_mfma_f32_16x16x32_f16 for the scores, v_mfma_f32_16x16x16_f16 for
+// the values.  Steps of 32 keys would use the matrix unit twice as well, which nothing here waits
+// for, and hold twice the registers: two workgroups per compute unit instead of four.
 template <int D>
 struct core_t<_Float16, D> {
-    static constexpr int KS = 32;     // keys per step
-    static constexpr int KL = 8;      // keys whose scores a lane holds
+    static constexpr int KS = 16;     // keys per step
+    static constexpr int KL = 4;      // keys whose scores a lane holds
     static constexpr int DV = D / 16; // elements of a row of V per lane
     static constexpr int QC = D / 32;
 
-    half8_t q[QC];
-    half8_t k[2][QC];
-    union vrow_t {
+    half8_t k[QC];
+    struct vrow_t {
         uint32_t u[DV / 2];
-        _Float16 h[DV];
     } v[KL];
 
-    static __device__ int key_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
+    static __device__ int key_of(int j, int g) { return 4 * g + j; }
 
     // PAD: d is below D.  Loads are unconditional (a branch around each would make it wait for
-    // the one before); elements beyond d come from the row's start and are zeroed.
+    // the one before); elements beyond d come from the row's start and are zeroed.  The queries
+    // wait in LDS, lane by lane: every step reads them once.
+    typedef half8_t query_t;
     template <bool PAD>
-    __device__ void load_q(_Float16 const* row, int g, int d, float sign)
+    static __device__ void load_q(query_t (*q)[64], int lane, _Float16 const* row, int g, int d,
+                                  float sign)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
             int const  e = c * 32 + g * 8;
             bool const in = !PAD || e < d;
-            q[c] = *reinterpret_cast<half8_t const*>(row + (in ? e : 0)) * _Float16(sign);
-            if (PAD && !in) q[c] = half8_t{};
+            half8_t const x = *reinterpret_cast<half8_t const*>(row + (in ? e : 0)) * _Float16(sign);
+            q[c][lane] = PAD && !in ? half8_t{} : x;
         }
     }
-    // element offsets of the two keys this lane loads of K, the eight of V; negative ones (no
-    // such entry) read the cache's first, to be masked by the caller
+    // element offsets of the key this lane loads of K, the four of V; negative ones (no such
+    // entry) read the cache's first, to be masked by the caller
     template <bool PAD>
-    __device__ void load(_Float16 const* kb, _Float16 const* vb, int64_t const* off, int c, int g,
-                         int d)
+    __device__ void load_k(_Float16 const* kb, int64_t const* off, int c, int g, int d)
     {
-        int64_t ok[2], ov[KL];
+        _Float16 const* p = kb + max(off[c], int64_t(0));
 #pragma unroll
-        for (int t = 0; t != 2; ++t) ok[t] = off[16 * t + c];
+        for (int i = 0; i != QC; ++i) {
+            int const e = i * 32 + g * 8;
+            k[i] = *reinterpret_cast<half8_t const*>(p + (!PAD || e < d ? e : 0));
+        }
+    }
+    template <bool PAD>
+    __device__ void load_v(_Float16 const* vb, int64_t const* off, int c, int g, int d)
+    {
+        int64_t ov[KL];
 #pragma unroll
         for (int j = 0; j != KL; ++j) ov[j] = off[key_of(j, g)];
-#pragma unroll
-        for (int t = 0; t != 2; ++t) {
-            _Float16 const* p = kb + max(ok[t], int64_t(0));
-#pragma unroll
-            for (int i = 0; i != QC; ++i) {
-                int const e = i * 32 + g * 8;
-                k[t][i] = *reinterpret_cast<half8_t const*>(p + (!PAD || e < d ? e : 0));
-            }
-        }
         constexpr int N = DV < 8 ? DV : 8;  // d is a multiple of 8
         typedef uint32_t vec_t __attribute__((ext_vector_type(N / 2)));
 #pragma unroll
@@ -411,18 +412,25 @@ struct core_t<_Float16, D> {
                 for (int i = 0; i != N / 2; ++i) v[j].u[e / 2 + i] = x[i];
             }
         }
-        if (PAD) {
+    }
+    // zeros beyond d, once the loads are there
+    template <bool PAD>
+    __device__ void trim_k(int g, int d)
+    {
+        if (!PAD) return;
 #pragma unroll
-            for (int i = 0; i != QC; ++i) {
-                if (i * 32 + g * 8 >= d) k[0][i] = k[1][i] = half8_t{};
-            }
+        for (int i = 0; i != QC; ++i) {
+            if (i * 32 + g * 8 >= d) k[i] = half8_t{};
+        }
+    }
+    template <bool PAD>
+    __device__ void trim_v(int c, int d)
+    {
+        if (!PAD) return;
 #pragma unroll
-            for (int j = 0; j != KL; ++j) {
+        for (int j = 0; j != KL; ++j) {
 #pragma unroll
-                for (int i = 0; i != DV / 2; ++i) {
-                    v[j].u[i] = c * DV + 2 * i < d ? v[j].u[i] : 0;
-                }
-            }
+            for (int i = 0; i != DV / 2; ++i) v[j].u[i] = c * DV + 2 * i < d ? v[j].u[i] : 0;
         }
     }
     __device__ void keep_key(int j, bool keep)
@@ -430,59 +438,48 @@ struct core_t<_Float16, D> {
 #pragma unroll
         for (int i = 0; i != DV / 2; ++i) v[j].u[i] = keep ? v[j].u[i] : 0;
     }
-    __device__ bool not_finite(int j) const
+    // zeros for what is not finite; true: there was some
+    __device__ bool clean_key(int j)
     {
-        bool bad = false;
+        uint32_t bad = 0;
 #pragma unroll
         for (int i = 0; i != DV / 2; ++i) {
-            bad |= (v[j].u[i] & 0x7c00u) == 0x7c00u || (v[j].u[i] & 0x7c000000u) == 0x7c000000u;
+            uint32_t const u = v[j].u[i];
+            uint32_t const cut = ((u & 0x7c00u) == 0x7c00u ? 0xffffu : 0) |
+                                 ((u & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0);
+            v[j].u[i] = u & ~cut;
+            bad |= cut;
         }
-        return bad;
+        return bad != 0;
     }
-    __device__ void scores(float* s) const
+    __device__ void scores(float* s, query_t const (*q)[64], int lane) const
     {
+        float4_t a = {0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t != 2; ++t) {
-            float4_t a = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i != QC; ++i) {
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][i], q[i], a, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r != 4; ++r) s[4 * t + r] = a[r];
+        for (int i = 0; i != QC; ++i) {
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], q[i][lane], a, 0, 0, 0);
         }
+#pragma unroll
+        for (int r = 0; r != 4; ++r) s[r] = a[r];
     }
-    // o[t] += V^T P^T for the elements i * DV + t of the head, i the result's row.  With ONLY:
-    // for the lanes with `take`, and with the keys whose bit is missing in `seen` as zeros.
-    template <bool ONLY>
-    __device__ void values(float const* p, float4_t* o, uint32_t seen, bool take) const
+    // o[t] += V^T P^T for the elements i * DV + t of the head, i the result's row
+    __device__ void values(float const* p, float4_t* o) const
     {
-        half8_t b;
+        half4_t b;
 #pragma unroll
         for (int j = 0; j != KL; ++j) b[j] = _Float16(p[j]);
 #pragma unroll
         for (int t = 0; t != DV; ++t) {
             union {
-                uint32_t u[4];
-                half8_t  h;
+                uint32_t u[2];
+                half4_t  h;
             } a;
             uint32_t const sel = t & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
-            for (int i = 0; i != 4; ++i) {
-                uint32_t lo = v[2 * i].u[t / 2], hi = v[2 * i + 1].u[t / 2];
-                if (ONLY) {
-                    lo = seen >> (2 * i) & 1 ? lo : 0;
-                    hi = seen >> (2 * i + 1) & 1 ? hi : 0;
-                }
-                a.u[i] = __builtin_amdgcn_perm(hi, lo, sel);
+            for (int i = 0; i != 2; ++i) {
+                a.u[i] = __builtin_amdgcn_perm(v[2 * i + 1].u[t / 2], v[2 * i].u[t / 2], sel);
             }
-            if (ONLY) {
-                float4_t const x =
-                    __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b, float4_t{0, 0, 0, 0}, 0, 0, 0);
-                if (take) o[t] += x;
-            } else {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b, o[t], 0, 0, 0);
-            }
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, b, o[t], 0, 0, 0);
         }
     }
 };
@@ -496,36 +493,41 @@ struct core_t<float, D> {
     static constexpr int DV = D / 16;
     static constexpr int QC = D / 16;
 
-    float4_t q[QC];
     float4_t k[QC];
     float    v[KL][DV];
 
     static __device__ int key_of(int j, int g) { return 4 * g + j; }
 
+    typedef float4_t query_t;
     template <bool PAD>
-    __device__ void load_q(float const* row, int g, int d, float sign)
+    static __device__ void load_q(query_t (*q)[64], int lane, float const* row, int g, int d,
+                                  float sign)
     {
 #pragma unroll
         for (int c = 0; c != QC; ++c) {
             int const  e = c * 16 + g * 4;
             bool const in = !PAD || e < d;
-            q[c] = *reinterpret_cast<float4_t const*>(row + (in ? e : 0)) * sign;
-            if (PAD && !in) q[c] = float4_t{};
+            float4_t const x = *reinterpret_cast<float4_t const*>(row + (in ? e : 0)) * sign;
+            q[c][lane] = PAD && !in ? float4_t{} : x;
         }
     }
     template <bool PAD>
-    __device__ void load(float const* kb, float const* vb, int64_t const* off, int c, int g, int d)
+    __device__ void load_k(float const* kb, int64_t const* off, int c, int g, int d)
     {
         int64_t const ok = off[c];
-        int64_t       ov[KL];
-#pragma unroll
-        for (int j = 0; j != KL; ++j) ov[j] = off[key_of(j, g)];
-        float const* p = kb + max(ok, int64_t(0));
+        float const*  p = kb + max(ok, int64_t(0));
 #pragma unroll
         for (int i = 0; i != QC; ++i) {
             int const e = i * 16 + g * 4;
             k[i] = *reinterpret_cast<float4_t const*>(p + (!PAD || e < d ? e : 0));
         }
+    }
+    template <bool PAD>
+    __device__ void load_v(float const* vb, int64_t const* off, int c, int g, int d)
+    {
+        int64_t ov[KL];
+#pragma unroll
+        for (int j = 0; j != KL; ++j) ov[j] = off[key_of(j, g)];
 #pragma unroll
         for (int j = 0; j != KL; ++j) {
             float const* pv = vb + max(ov[j], int64_t(0));
@@ -537,16 +539,24 @@ struct core_t<float, D> {
                 for (int i = 0; i != 4; ++i) v[j][e + i] = x[i];
             }
         }
-        if (PAD) {
+    }
+    template <bool PAD>
+    __device__ void trim_k(int g, int d)
+    {
+        if (!PAD) return;
 #pragma unroll
-            for (int i = 0; i != QC; ++i) {
-                if (i * 16 + g * 4 >= d) k[i] = float4_t{};
-            }
+        for (int i = 0; i != QC; ++i) {
+            if (i * 16 + g * 4 >= d) k[i] = float4_t{};
+        }
+    }
+    template <bool PAD>
+    __device__ void trim_v(int c, int d)
+    {
+        if (!PAD) return;
 #pragma unroll
-            for (int j = 0; j != KL; ++j) {
+        for (int j = 0; j != KL; ++j) {
 #pragma unroll
-                for (int e = 0; e != DV; ++e) v[j][e] = c * DV + e < d ? v[j][e] : 0.0f;
-            }
+            for (int e = 0; e != DV; ++e) v[j][e] = c * DV + e < d ? v[j][e] : 0.0f;
         }
     }
     __device__ void keep_key(int j, bool keep)
@@ -554,43 +564,38 @@ struct core_t<float, D> {
 #pragma unroll
         for (int i = 0; i != DV; ++i) v[j][i] = keep ? v[j][i] : 0.0f;
     }
-    __device__ bool not_finite(int j) const
+    __device__ bool clean_key(int j)
     {
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i != DV; ++i) {
-            bad |= (__builtin_bit_cast(uint32_t, v[j][i]) & 0x7f800000u) == 0x7f800000u;
+        for (int e = 0; e != DV; ++e) {
+            bool const fine = v[j][e] - v[j][e] == 0.0f;
+            v[j][e] = fine ? v[j][e] : 0.0f;
+            bad |= !fine;
         }
         return bad;
     }
-    __device__ void scores(float* s) const
+    __device__ void scores(float* s, query_t const (*q)[64], int lane) const
     {
         float4_t a = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i != QC; ++i) {
+            float4_t const x = q[i][lane];
 #pragma unroll
             for (int e = 0; e != 4; ++e) {
-                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][e], q[i][e], a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][e], x[e], a, 0, 0, 0);
             }
         }
 #pragma unroll
         for (int r = 0; r != 4; ++r) s[r] = a[r];
     }
-    template <bool ONLY>
-    __device__ void values(float const* p, float4_t* o, uint32_t seen, bool take) const
+    __device__ void values(float const* p, float4_t* o) const
     {
 #pragma unroll
         for (int t = 0; t != DV; ++t) {
-            float4_t x = ONLY ? float4_t{0, 0, 0, 0} : o[t];
 #pragma unroll
             for (int j = 0; j != KL; ++j) {
-                float const e = !ONLY || (seen >> j & 1) ? v[j][t] : 0.0f;
-                x = __builtin_amdgcn_mfma_f32_16x16x4f32(e, p[j], x, 0, 0, 0);
-            }
-            if (!ONLY) {
-                o[t] = x;
-            } else if (take) {
-                o[t] += x;
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j][t], p[j], o[t], 0, 0, 0);
             }
         }
     }
@@ -624,15 +629,19 @@ struct few_shared_t {
     static constexpr int DJ = D < 128 ? D : 128;  // elements joined at a time
     deal_t  deal;
     int     limit[FEW];
-    int64_t off[WAVES][32];
+    int64_t off[WAVES][2][16];
     float   m[WAVES][FEW], l[WAVES][FEW];
-    float   o[WAVES][FEW][DJ + 4];
+    union {
+        float                          o[WAVES][FEW][DJ + 4];
+        typename core_t<T, D>::query_t q[core_t<T, D>::QC][64];  // the same for every wavefront
+    };
 };
 
 // The workgroup's keys against the tile's rows; steps w, w + WAVES, ...
 template <typename T, int D, bool PAD>
-__device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const& wk, row_t const& row,
-                           int least, int kvh, float4_t* o, float& m, float& l)
+__device__ void attend_few(attention_dev_t const& a, int64_t (*offs)[16],
+                           typename core_t<T, D>::query_t const (*q)[64], work_t const& wk,
+                           row_t const& row, int least, int kvh, float4_t* o, float& m, float& l)
 {
     typedef core_t<T, D> core;
     constexpr int        KS = core::KS, KL = core::KL, DV = core::DV;
@@ -642,18 +651,13 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
     T const* const       kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
     T const* const       vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
     core                 x;
-    // a column without a row computes what nobody stores
-    x.template load_q<PAD>(reinterpret_cast<T const*>(a.q) +
-                               uint64_t(max(row.token, 0)) * a.q_stride +
-                               uint64_t(row.head) * uint64_t(a.d),
-                           g, a.d, a.q_sign);
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
-    // a step ahead: the page of this lane's key (-1: not among them, or no such page)
+    // two steps ahead: the page of this lane's key (-1: not among them, or no such page)
     int  page = -1, prow = 0;
-    auto look_up = [&](int base) {
-        int const pos = base + (lane & (KS - 1));
+    auto look_up = [&](int at) {
+        int const pos = at + (lane & (KS - 1));
         page = -1;
         if (pos >= lo && pos < hi) {
             int const pi = page_of(a, pos);
@@ -661,22 +665,40 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             page = wk.table[pi];
         }
     };
-    int   base = (lo / KS + w) * KS;
-    float ref = 0;
-    look_up(base);
-    for (; base < hi; base += WAVES * KS) {
+    // where the looked-up keys lie, for all lanes; true: some are nowhere
+    auto place = [&](int64_t* off) {
         int64_t const at = entry_of(a, page, prow);
-        bool const    holes = __any(at < 0);
         __builtin_amdgcn_wave_barrier();
         if (lane < KS) off[lane] = at;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        look_up(base + WAVES * KS);
-        x.template load<PAD>(kb, vb, off, c, g, a.d);
-        // all of the step's loads go out before the first is waited for
+        return bool(__any(at < 0));
+    };
+    constexpr int STEP = WAVES * KS;
+    int           base = (lo / KS + w) * KS;
+    float         ref = 0;
+    bool          bad = false;
+    look_up(base);
+    bool holes = place(offs[0]), holes_next = false;
+    look_up(base + STEP);
+    x.template load_k<PAD>(kb, offs[0], c, g, a.d);
+    x.template load_v<PAD>(vb, offs[0], c, g, a.d);
+    // The next step's K is asked for as soon as this step's scores are computed, its V after this
+    // step's values: a wavefront always has one of the two on its way.  Behind the last step, too
+    // (positions that are not there read the cache's first entry): loads under a condition made
+    // the compiler take registers of V for free.
+    for (int turn = 0; base < hi; base += STEP, turn ^= 1) {
+        int64_t const* const off = offs[turn];
+        holes_next = place(offs[turn ^ 1]);
+        look_up(base + 2 * STEP);
         __builtin_amdgcn_sched_barrier(0);
+        x.template trim_k<PAD>(g, a.d);
         float s[KL];
-        x.scores(s);
+        x.scores(s, q, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        x.template load_k<PAD>(kb, offs[turn ^ 1], c, g, a.d);
+        __builtin_amdgcn_sched_barrier(0);
+        x.template trim_v<PAD>(c, a.d);
         bool const edge = holes || base + KS - 1 > seen_by_all;
         uint32_t   masked = 0;
         if (edge) {
@@ -684,7 +706,10 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             for (int j = 0; j != KL; ++j) {
                 int const  key = core::key_of(j, g);
                 bool const hole = off[key] < 0;
+                // zero times an infinity or NaN is no zero: such values become zeros here and are
+                // added in the end to the rows that see them
                 x.keep_key(j, !hole);
+                bad |= x.clean_key(j);
                 masked |= hole || base + key > row.limit ? 1u << j : 0;
             }
         }
@@ -702,26 +727,27 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
             sum += s[j];
         }
         l += sum;
-        // Zero times an infinity or NaN is no zero: where a row may not see a key whose values
-        // are not finite, the rows are taken one by one, each with the keys it sees.
-        bool careful = false;
-        if (edge) {
-            bool bad = false;
+        x.values(s, o);
+        __builtin_amdgcn_sched_barrier(0);
+        x.template load_v<PAD>(vb, offs[turn ^ 1], c, g, a.d);
+        holes = holes_next;
+    }
+    if (__any(bad)) {
+        for (base = (lo / KS + w) * KS; base < hi; base += STEP) {
+            for (int pos = max(base, lo); pos < min(base + KS, hi); ++pos) {
+                int const     pi = page_of(a, pos);
+                int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
+                if (at < 0) continue;
 #pragma unroll
-            for (int j = 0; j != KL; ++j) bad |= x.not_finite(j);
-            careful = __any(bad);
-        }
-        if (!careful) {
-            x.template values<false>(s, o, 0, true);
-        } else {
-            for (int r = 0; r != FEW; ++r) {
-                int const limit = __shfl(row.limit, r);
-                uint32_t  seen = 0;
+                for (int t = 0; t != DV; ++t) {
 #pragma unroll
-                for (int j = 0; j != KL; ++j) {
-                    if (base + core::key_of(j, g) <= limit) seen |= 1u << j;
+                    for (int r = 0; r != 4; ++r) {
+                        int const   e = (4 * g + r) * DV + t;
+                        float const y = float(vb[at + (!PAD || e < a.d ? e : 0)]);
+                        bool const  add = !(y - y == 0.0f) && (!PAD || e < a.d);
+                        o[t][r] += add && pos <= row.limit ? y : 0.0f;
+                    }
                 }
-                x.template values<true>(s, o, seen, c == r);
             }
         }
     }
@@ -730,7 +756,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off, work_t const&
 }
 
 template <typename T, int D, bool PAD>
-__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kernel(attention_dev_t a)
+__global__ __launch_bounds__(THREADS, D == 256 ? 2 : D == 128 && sizeof(T) == 4 ? 3 : 4) void attention_few_kernel(attention_dev_t a)
 {
     __shared__ few_shared_t<T, D> sh;
     int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
@@ -749,7 +775,17 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_few_kerne
 #pragma unroll
     for (int t = 0; t != DV; ++t) o[t] = float4_t{0, 0, 0, 0};
     float m = NEG_INF, l = 0;
-    if (wk.lo < wk.hi) attend_few<T, D, PAD>(a, sh.off[w], wk, row, least, kvh, o, m, l);
+    // a column without a row computes what nobody stores
+    if (w == 0) {
+        core_t<T, D>::template load_q<PAD>(sh.q, lane,
+                                           reinterpret_cast<T const*>(a.q) +
+                                               uint64_t(max(row.token, 0)) * a.q_stride +
+                                               uint64_t(row.head) * uint64_t(a.d),
+                                           g, a.d, a.q_sign);
+    }
+    __syncthreads();
+    if (wk.lo < wk.hi) attend_few<T, D, PAD>(a, sh.off[w], sh.q, wk, row, least, kvh, o, m, l);
+    __syncthreads();  // the queries' place is used again
 
     // join the wavefronts
     if (g == 0) {
