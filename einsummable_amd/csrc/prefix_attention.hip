@@ -62,13 +62,14 @@ struct attention_dev_t {
     float       q_sign;  // -1, 0 or 1, multiplied into q: the sign of the caller's scale
     uint32_t    page_magic, page_shift;
     int         prefix_tiles, prefix_splits, prefix_chunk, prefix_rows;
-    int         split_target;
-    int         items, own_rows;
+    int         shares;     // parts that the own positions of the whole batch are cut into
+    int         grain;      // steps per unit of work of the few-row kernel
+    int         own_slots, own_rows;
     int         parts;      // what this launch does: 1 prefix, 2 own positions, 3 both
     int         direct;     // there are no shared positions to join with
     float*      part_o;     // [row of a slot][D]: the prefix's slots, then the own ones
     float*      part_ml;    // [row of a slot][2]
-    int*        part_meta;  // [token][4]: first cut of the sequence's first tile, cuts, token 0
+    int4*       part_meta;  // [token * group + head of the group], see piece()
     int64_t     own_base;   // rows before the own positions' slots
 };
 
@@ -85,14 +86,6 @@ __device__ inline int wave_scan(int v)
     v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast:15
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // row_bcast:31
-    return v;
-}
-
-// Sum over the 64 lanes, in every lane; the same additions whatever the wavefront.
-__device__ inline float wave_sum(float v)
-{
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
@@ -130,8 +123,8 @@ __device__ inline int64_t entry_of(attention_dev_t const& a, int page, int row)
     return int64_t(uint64_t(page) * a.page_stride + uint64_t(row) * a.token_stride);
 }
 
-// What a workgroup was given: the positions lo <= p < hi of a page table's row, and a tile of
-// rows, which are either rows of the whole batch or of one sequence.
+// What a workgroup works at: the positions lo <= p < hi of a page table's row, and a tile of rows,
+// which are either rows of the whole batch or of one sequence.
 struct work_t {
     int        lo, hi;
     int const* table;
@@ -150,37 +143,37 @@ struct row_t {
     int limit = 0x7fffffff;  // its last position
 };
 
-struct deal_t {
-    float total[WAVES];
-    int   before[WAVES];
-    int   found[8];  // sequence, item within it, first item, cuts, offsets, length
-};
-
-template <int ROWS>
-__device__ inline row_t row_of(attention_dev_t const& a, work_t const& k, int const* limit, int kvh,
-                               int i)
+// Row i of the tile, all but its limit.
+__device__ inline row_t row_of(attention_dev_t const& a, work_t const& k, int kvh, int i)
 {
     row_t     row;
     int const r = k.r0 + i;
     int const j = r / a.group;
     int const t = k.b + j;
     if (t >= k.e) return row;
-    int at;
-    if (k.whole) {
-        at = limit[j - k.r0 / a.group];
-        if (at == -2) return row;
-    } else {
-        at = max(k.len - (k.end - t), -1);
-    }
     row.token = t;
     row.head = kvh * a.group + r - j * a.group;
-    row.limit = at;
     return row;
 }
 
+__device__ inline void set_limit(attention_dev_t const& a, work_t const& k, int const* limit,
+                                 row_t& row)
+{
+    if (row.token < 0) return;
+    if (!k.whole) {
+        row.limit = max(k.len - (k.end - row.token), -1);
+        return;
+    }
+    int const at = limit[row.token - k.r0 / a.group];
+    if (at == -2) {
+        row.token = -1;  // of no sequence
+    } else {
+        row.limit = at;
+    }
+}
+
 // Workgroups go to the eight XCDs in turn.  The heads of one unit (a row tile and a cut) stay on
-// one XCD: together they read whole rows of the cache, while one head per XCD would ask its L2
-// for 256 bytes every n_kv_heads * 256, which few of its channels hold.
+// one XCD: together they read whole rows of the cache.
 __device__ inline void unit_of_block(attention_dev_t const& a, int& unit, int& kvh)
 {
     int const xcd = int(blockIdx.x) & 7, i = int(blockIdx.x) >> 3;
@@ -188,159 +181,218 @@ __device__ inline void unit_of_block(attention_dev_t const& a, int& unit, int& k
     unit = i / a.h_kv * 8 + xcd;
 }
 
-// Finds the workgroup's work; false: there is none.  `limit` holds ROWS ints.
-template <int ROWS, int KS>
-__device__ bool deal(attention_dev_t const& a, deal_t& sh, int* limit, int unit, int kvh, work_t& k)
+// A prefix workgroup: a tile of the batch's rows against a cut of the shared positions.
+template <int ROWS>
+__device__ inline void deal_prefix(attention_dev_t const& a, int unit, int kvh, work_t& k)
 {
-    int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
-    int const prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
-    int const reach = a.max_pages * a.page_size;  // positions that a table row has pages for
-    if (unit < prefix_units) {
-        int const tile = unit % a.prefix_tiles;
-        int const split = unit / a.prefix_tiles;
-        k.part = (int64_t(unit) * a.h_kv + kvh) * ROWS;
-        k.lo = split * a.prefix_chunk;
-        k.hi = min(min(k.lo + a.prefix_chunk, a.shared), reach);
-        k.table = a.table;
-        k.direct = false;
-        k.whole = true;
-        k.r0 = tile * ROWS;
-        k.b = 0;
-        int const t0 = k.r0 / a.group;
-        k.e = min((k.r0 + ROWS - 1) / a.group + 1, a.n_tokens);
-        k.end = k.len = 0;
-        for (int i = tid; i < ROWS; i += THREADS) limit[i] = -2;
-        __syncthreads();
-        // each thread puts down the positions of the tile's tokens in its sequences
-        for (int s = tid; s < a.n_seqs; s += THREADS) {
-            int const b = a.offsets[s], e = a.offsets[s + 1];
-            int const len = a.lens[s];
-            for (int t = max(b, t0); t < min(e, k.e); ++t) {
-                limit[t - t0] = max(len - (e - t), -1);
-            }
-        }
-        __syncthreads();
-        return true;
+    int const tile = unit % a.prefix_tiles;
+    int const split = unit / a.prefix_tiles;
+    k.part = (int64_t(unit) * a.h_kv + kvh) * ROWS;
+    k.lo = split * a.prefix_chunk;
+    k.hi = min(min(k.lo + a.prefix_chunk, a.shared), a.max_pages * a.page_size);
+    k.table = a.table;
+    k.direct = false;
+    k.whole = true;
+    k.r0 = tile * ROWS;
+    k.b = 0;
+    k.e = min((k.r0 + ROWS - 1) / a.group + 1, a.n_tokens);
+    k.end = k.len = 0;
+}
+
+// Puts down the positions of the tile's tokens in their sequences (-2: of none); `limit` holds
+// ROWS ints.  Ends with a barrier.
+template <int ROWS>
+__device__ inline void prefix_limits(attention_dev_t const& a, work_t const& k, int* limit)
+{
+    int const tid = int(threadIdx.x), t0 = k.r0 / a.group;
+    for (int i = tid; i < ROWS; i += THREADS) limit[i] = -2;
+    __syncthreads();
+    for (int s = tid; s < a.n_seqs; s += THREADS) {
+        int const b = a.offsets[s], e = a.offsets[s + 1];
+        int const len = a.lens[s];
+        for (int t = max(b, t0); t < min(e, k.e); ++t) limit[t - t0] = max(len - (e - t), -1);
     }
-    // The cuts of all sequences, numbered through: tiles_s * splits_s each, where a cut holds
-    // `chunk` steps.  Up to 64 sequences every wavefront adds up for itself, one per lane;
-    // more are dealt to the threads in runs.
-    int const item = unit - prefix_units;
-    if (item >= a.items) return false;
-    int  sb = 0, se = 0, slen = 0;
-    auto tiles_steps = [&](int s, int& tiles, int& steps) {
-        sb = a.offsets[s];
-        se = a.offsets[s + 1];
-        slen = a.lens[s];
-        int const b = max(sb, 0), e = min(se, a.n_tokens);
-        int const len = min(slen, reach);
-        tiles = e > b ? ((e - b) * a.group + ROWS - 1) / ROWS : 0;
-        steps = len > a.shared ? (len + KS - 1) / KS - a.shared / KS : 0;
-    };
-    // Steps per cut, a multiple of four: one for each wavefront that takes them in turn.  The sum
-    // is taken in fp32, so 2^-10 of it and one step are added: the cuts never number more than the
-    // grid was made for.
-    auto steps_per_cut = [&](float all) {
-        if (a.split_target <= 0) return 0x3fffffff;
-        float const per = all / float(a.split_target) * (1.0f + 0x1p-10f) + 1.0f;
-        return int(fminf(per, 1e9f)) / WAVES * WAVES + WAVES;
-    };
-    auto cuts = [](int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); };
-    int  s, index, first_item, splits, chunk, seq_b, seq_e, seq_len;
+    __syncthreads();
+}
+
+// ---- the sequences' own positions
+//
+// Work is counted in units: a tile of rows (ROWS queries of one sequence) times `grain` steps of
+// KS positions, at least one per tile.  A tile is cut into pieces of `each` units, so that the
+// batch has about `shares` of them, and what is left over; a piece to a workgroup.  The whole
+// pieces are numbered first, the rests behind them: workgroups start in this order, so the short
+// ones fill the gaps at the end.  All of it follows from the lengths in device memory, and every
+// workgroup works it out for itself: up to 64 sequences a wavefront does, one per lane; more are
+// dealt to the threads in runs.
+struct deal_t {
+    int sums[3][WAVES];
+    int found[8];
+};
+
+struct sequence_t {
+    int s, b, e, len;
+    int per;            // units per tile
+    int whole0, rest0;  // number of its first whole piece, of its first rest
+};
+
+// Tiles of a sequence and units per tile.
+template <int ROWS, int KS>
+__device__ inline void measure(attention_dev_t const& a, int b, int e, int len, int& tiles, int& per)
+{
+    int const first = max(b, 0), last = min(e, a.n_tokens);
+    int const reach = min(len, a.max_pages * a.page_size);
+    int const steps = reach > a.shared ? (reach + KS - 1) / KS - a.shared / KS : 0;
+    tiles = last > first ? ((last - first) * a.group + ROWS - 1) / ROWS : 0;
+    per = max(1, (steps + a.grain - 1) / a.grain);
+}
+
+// Units per piece.  A multiple of four steps: one for each wavefront that takes them in turn.
+__device__ inline int units_per_piece(attention_dev_t const& a, int total)
+{
+    if (a.shares == 0) return 0x3fffffff;
+    int const each = max(1, (total + a.shares - 1) / a.shares);
+    return a.grain % WAVES ? (each + WAVES - 1) / WAVES * WAVES : each;
+}
+
+// The piece that `item` numbers; false: there is none.  The same in all lanes.
+template <int ROWS, int KS>
+__device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int item, work_t& k)
+{
+    if (item >= a.own_slots) return false;
+    int const  tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
+    sequence_t q;
+    int        each, wholes;  // units per piece, whole pieces in all
     if (a.n_seqs <= 64) {
-        int tiles = 0, steps = 0;
-        if (lane < a.n_seqs) tiles_steps(lane, tiles, steps);
-        chunk = __builtin_amdgcn_readfirstlane(
-            steps_per_cut(wave_sum(float(tiles) * float(steps))));
-        int const      each = cuts(steps, chunk);
-        int const      mine = tiles * each;
-        int const      start = wave_scan(mine) - mine;
-        uint64_t const here = __ballot(item >= start && item < start + mine);
+        int sb = 0, se = 0, slen = 0, tiles = 0, per = 1;
+        if (lane < a.n_seqs) {
+            sb = a.offsets[lane];
+            se = a.offsets[lane + 1];
+            slen = a.lens[lane];
+            measure<ROWS, KS>(a, sb, se, slen, tiles, per);
+        }
+        each = units_per_piece(a, __builtin_amdgcn_readlane(wave_scan(tiles * per), 63));
+        int const whole = tiles * (per / each), rest = tiles * (per % each != 0);
+        int const whole_n = wave_scan(whole), rest_n = wave_scan(rest);
+        wholes = __builtin_amdgcn_readlane(whole_n, 63);
+        int const      at = item < wholes ? item : item - wholes;
+        int const      mine = item < wholes ? whole : rest;
+        int const      start = (item < wholes ? whole_n : rest_n) - mine;
+        uint64_t const here = __ballot(at >= start && at < start + mine);
         if (here == 0) return false;
-        s = __ffsll((unsigned long long)here) - 1;
-        first_item = __builtin_amdgcn_readlane(start, s);
-        splits = __builtin_amdgcn_readlane(each, s);
-        seq_b = __builtin_amdgcn_readlane(sb, s);
-        seq_e = __builtin_amdgcn_readlane(se, s);
-        seq_len = __builtin_amdgcn_readlane(slen, s);
-        index = item - first_item;
+        int const s = __ffsll((unsigned long long)here) - 1;
+        q.s = s;
+        q.b = __builtin_amdgcn_readlane(sb, s);
+        q.e = __builtin_amdgcn_readlane(se, s);
+        q.len = __builtin_amdgcn_readlane(slen, s);
+        q.per = __builtin_amdgcn_readlane(per, s);
+        q.whole0 = __builtin_amdgcn_readlane(whole_n - whole, s);
+        q.rest0 = __builtin_amdgcn_readlane(rest_n - rest, s);
     } else {
         int const run = (a.n_seqs + THREADS - 1) / THREADS;
         int const s0 = min(tid * run, a.n_seqs), s1 = min(s0 + run, a.n_seqs);
+        int       b = 0, e = 0, len = 0, tiles = 0, per = 1, units = 0;
+        auto      read = [&](int s) {
+            b = a.offsets[s];
+            e = a.offsets[s + 1];
+            len = a.lens[s];
+            measure<ROWS, KS>(a, b, e, len, tiles, per);
+        };
+        for (int s = s0; s < s1; ++s) {
+            read(s);
+            units += tiles * per;
+        }
+        units = wave_scan(units);
+        if (lane == 63) sh.sums[0][w] = units;
         if (tid == 0) sh.found[0] = -1;
-        float total = 0;
-        int   tiles = 0, steps = 0;
-        for (int i = s0; i < s1; ++i) {
-            tiles_steps(i, tiles, steps);
-            total += float(tiles) * float(steps);
-        }
-        total = wave_sum(total);
-        if (lane == 0) sh.total[w] = total;
         __syncthreads();
-        chunk = steps_per_cut(sh.total[0] + sh.total[1] + sh.total[2] + sh.total[3]);
-        int mine = 0;
-        for (int i = s0; i < s1; ++i) {
-            if (run > 1) tiles_steps(i, tiles, steps);
-            mine += tiles * cuts(steps, chunk);
+        each = units_per_piece(a, sh.sums[0][0] + sh.sums[0][1] + sh.sums[0][2] + sh.sums[0][3]);
+        int whole = 0, rest = 0;
+        for (int s = s0; s < s1; ++s) {
+            if (run > 1) read(s);
+            whole += tiles * (per / each);
+            rest += tiles * (per % each != 0);
         }
-        int const incl = wave_scan(mine);
-        if (lane == 63) sh.before[w] = incl;
+        int const whole_n = wave_scan(whole), rest_n = wave_scan(rest);
+        if (lane == 63) {
+            sh.sums[1][w] = whole_n;
+            sh.sums[2][w] = rest_n;
+        }
         __syncthreads();
-        int start = incl - mine;
+        int whole0 = whole_n - whole, rest0 = rest_n - rest;
+        wholes = 0;
 #pragma unroll
-        for (int i = 0; i != WAVES; ++i) start += i < w ? sh.before[i] : 0;
-        if (item >= start && item < start + mine) {
-            for (int i = s0; i < s1; ++i) {
-                if (run > 1) tiles_steps(i, tiles, steps);
-                int const each = cuts(steps, chunk);
-                if (item < start + tiles * each) {
-                    sh.found[0] = i;
-                    sh.found[1] = item - start;
-                    sh.found[2] = start;
-                    sh.found[3] = each;
-                    sh.found[4] = sb;
-                    sh.found[5] = se;
-                    sh.found[6] = slen;
+        for (int i = 0; i != WAVES; ++i) {
+            whole0 += i < w ? sh.sums[1][i] : 0;
+            rest0 += i < w ? sh.sums[2][i] : 0;
+            wholes += sh.sums[1][i];
+        }
+        int const at = item < wholes ? item : item - wholes;
+        int const start = item < wholes ? whole0 : rest0, mine = item < wholes ? whole : rest;
+        if (at >= start && at < start + mine) {
+            for (int s = s0; s < s1; ++s) {
+                if (run > 1) read(s);
+                int const n = tiles * (per / each), r = tiles * (per % each != 0);
+                if (at < (item < wholes ? whole0 + n : rest0 + r)) {
+                    sh.found[0] = s;
+                    sh.found[1] = b;
+                    sh.found[2] = e;
+                    sh.found[3] = len;
+                    sh.found[4] = per;
+                    sh.found[5] = whole0;
+                    sh.found[6] = rest0;
                     break;
                 }
-                start += tiles * each;
+                whole0 += n;
+                rest0 += r;
             }
         }
         __syncthreads();
-        s = __builtin_amdgcn_readfirstlane(sh.found[0]);
-        if (s < 0) return false;
-        index = __builtin_amdgcn_readfirstlane(sh.found[1]);
-        first_item = __builtin_amdgcn_readfirstlane(sh.found[2]);
-        splits = __builtin_amdgcn_readfirstlane(sh.found[3]);
-        seq_b = __builtin_amdgcn_readfirstlane(sh.found[4]);
-        seq_e = __builtin_amdgcn_readfirstlane(sh.found[5]);
-        seq_len = __builtin_amdgcn_readfirstlane(sh.found[6]);
+        q.s = __builtin_amdgcn_readfirstlane(sh.found[0]);
+        if (q.s < 0) return false;
+        q.b = __builtin_amdgcn_readfirstlane(sh.found[1]);
+        q.e = __builtin_amdgcn_readfirstlane(sh.found[2]);
+        q.len = __builtin_amdgcn_readfirstlane(sh.found[3]);
+        q.per = __builtin_amdgcn_readfirstlane(sh.found[4]);
+        q.whole0 = __builtin_amdgcn_readfirstlane(sh.found[5]);
+        q.rest0 = __builtin_amdgcn_readfirstlane(sh.found[6]);
+        wholes = __builtin_amdgcn_readfirstlane(wholes);
+        each = __builtin_amdgcn_readfirstlane(each);
     }
-    int const tile = index / splits, split = index - tile * splits;
-    k.b = max(seq_b, 0);
-    k.e = min(seq_e, a.n_tokens);
-    k.end = seq_e;
-    k.len = seq_len;
+    int const n = q.per / each, rest = q.per - n * each;
+    int       tile, at;
+    if (item < wholes) {
+        tile = (item - q.whole0) / n;
+        at = (item - q.whole0 - tile * n) * each;
+    } else {
+        tile = item - wholes - q.rest0;
+        at = n * each;
+    }
+    k.b = max(q.b, 0);
+    k.e = min(q.e, a.n_tokens);
+    k.end = q.e;
+    k.len = q.len;
     k.whole = false;
     k.part = a.own_base + (int64_t(item) * a.h_kv + kvh) * ROWS;
-    k.direct = splits == 1 && a.direct;
-    k.table = a.table + uint64_t(s) * a.table_stride;
+    int const parts = n + (rest != 0);
+    k.direct = parts == 1 && a.direct;
+    k.table = a.table + uint64_t(q.s) * a.table_stride;
     k.r0 = tile * ROWS;
-    int const last = min(k.e - 1, k.b + (k.r0 + ROWS - 1) / a.group);
-    if (split == 0 && kvh == 0) {
-        int const first = k.b + k.r0 / a.group;
-        for (int t = first + tid; t <= last; t += THREADS) {
-            int* const meta = a.part_meta + 4 * t;
-            meta[0] = first_item;
-            meta[1] = k.direct ? 0 : splits;
-            meta[2] = k.b;
+    if (at == 0 && kvh == 0) {
+        // where the rows' partial results are: from x on y of them, then z (or none); w the row
+        for (int i = tid; i < ROWS; i += THREADS) {
+            int const r = k.r0 + i, t = k.b + r / a.group;
+            if (t < k.e) {
+                a.part_meta[k.b * a.group + r] =
+                    int4{q.whole0 + tile * n, k.direct ? -1 : n,
+                         rest ? wholes + q.rest0 + tile : -1, i};
+            }
         }
     }
-    // positions of this cut, up to the last one that a row of the tile sees
-    int const len = min(k.len, reach);
-    int const step0 = a.shared / KS + (splits == 1 ? 0 : split * chunk);
+    int const last = min(k.e - 1, k.b + (k.r0 + ROWS - 1) / a.group);
+    // positions, up to the last one that a row of the tile sees
+    int const step0 = a.shared / KS + at * a.grain;
     k.lo = max(a.shared, step0 * KS);
-    k.hi = splits == 1 ? len : min(len, (step0 + chunk) * KS);
+    k.hi = min(min(k.len, a.max_pages * a.page_size), (step0 + min(each, q.per - at) * a.grain) * KS);
     k.hi = min(k.hi, k.len - (k.end - last) + 1);
     return true;
 }
@@ -761,17 +813,24 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 2 : D == 128 && sizeof(T) == 4 
     __shared__ few_shared_t<T, D> sh;
     int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
     int const c = lane & 15, g = lane >> 4;
-    int       unit, kvh;
+    constexpr int KS = core_t<T, D>::KS, DV = core_t<T, D>::DV;
+    int           unit, kvh;
     unit_of_block(a, unit, kvh);
-    work_t wk;
-    if (!deal<FEW, core_t<T, D>::KS>(a, sh.deal, sh.limit, unit, kvh, wk)) return;
-    row_t const row = row_of<FEW>(a, wk, sh.limit, kvh, c);
-    int         least = row.limit;
+    int const prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
+    work_t    wk;
+    if (unit < prefix_units) {
+        deal_prefix<FEW>(a, unit, kvh, wk);
+        prefix_limits<FEW>(a, wk, sh.limit);
+    } else if (!piece<FEW, KS>(a, sh.deal, kvh, unit - prefix_units, wk)) {
+        return;
+    }
+    row_t row = row_of(a, wk, kvh, c);
+    set_limit(a, wk, sh.limit, row);
+    int least = row.limit;
 #pragma unroll
     for (int i = 1; i != 16; i <<= 1) least = min(least, __shfl_xor(least, i));
 
-    constexpr int DV = core_t<T, D>::DV;
-    float4_t      o[DV];
+    float4_t o[DV];
 #pragma unroll
     for (int t = 0; t != DV; ++t) o[t] = float4_t{0, 0, 0, 0};
     float m = NEG_INF, l = 0;
@@ -939,8 +998,14 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     int const c = lane & 15, g = lane >> 4;
     int       unit, kvh;
     unit_of_block(a, unit, kvh);
-    work_t wk;
-    if (!deal<ROWS, 32>(a, sh.deal, sh.limit, unit, kvh, wk)) return;
+    int const  prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
+    bool const prefix = unit < prefix_units;
+    work_t     wk;
+    if (prefix) {
+        deal_prefix<ROWS>(a, unit, kvh, wk);
+    } else {
+        if (!piece<ROWS, KT>(a, sh.deal, kvh, unit - prefix_units, wk)) return;
+    }
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const first = lo / 32 * 32;
@@ -954,20 +1019,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     if (lo < hi) page0 = *page_at(position(0));
 
     row_t row[NT];
-    int   least = 0x7fffffff, most = -1;
 #pragma unroll
-    for (int n = 0; n != NT; ++n) {
-        row[n] = row_of<ROWS>(a, wk, sh.limit, kvh, (w * NT + n) * 16 + c);
-        least = min(least, row[n].limit);
-        if (row[n].token >= 0) most = max(most, row[n].limit);
-    }
-#pragma unroll
-    for (int i = 1; i != 16; i <<= 1) {
-        least = min(least, __shfl_xor(least, i));
-        most = max(most, __shfl_xor(most, i));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
+    for (int n = 0; n != NT; ++n) row[n] = row_of(a, wk, kvh, (w * NT + n) * 16 + c);
 
     half8_t  q[NT][D / 32];
     float4_t o[NT][DT + 1];  // [DT]: the sum of the weights, four times
@@ -995,6 +1048,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         char const* const vb = a.v + uint64_t(kvh) * a.head_stride * 2;
         char const* const zeros = reinterpret_cast<char const*>(attention_zeros);
         int const         tiles = (hi - first + KT - 1) / KT;
+        int               least = 0x7fffffff, most = -1;
 
         auto put_entry = [&](int n, int page) {
             int const pos = position(n);
@@ -1095,9 +1149,33 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         };
 
         if (tid == 0) sh.holes = sh.bad = 0;
-        if (lane == 0) sh.least[w] = least;
         __syncthreads();
         put_entry(0, page0);
+        __syncthreads();
+        load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
+        // beyond the last tile too: the waits count instructions (the entries are zeros)
+#pragma unroll
+        for (int i = 0; i != NS - 1; ++i) {
+            aim(i);
+            load_tile(i);
+        }
+        aim(NS - 1);
+        // while they are on their way: who sees what
+        if (prefix) prefix_limits<ROWS>(a, wk, sh.limit);
+#pragma unroll
+        for (int n = 0; n != NT; ++n) {
+            set_limit(a, wk, sh.limit, row[n]);
+            least = min(least, row[n].limit);
+            if (row[n].token >= 0) most = max(most, row[n].limit);
+        }
+#pragma unroll
+        for (int i = 1; i != 16; i <<= 1) {
+            least = min(least, __shfl_xor(least, i));
+            most = max(most, __shfl_xor(most, i));
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
+        if (lane == 0) sh.least[w] = least;
         __syncthreads();
         // the least limit of the workgroup's rows decides where values have to be looked at
         int const all_see = __builtin_amdgcn_readfirstlane(
@@ -1125,14 +1203,6 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             }
             __syncthreads();
         };
-        load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
-        // beyond the last tile too: the waits count instructions (the entries are zeros)
-#pragma unroll
-        for (int i = 0; i != NS - 1; ++i) {
-            aim(i);
-            load_tile(i);
-        }
-        aim(NS - 1);
         wait_loads<2 * LPT*(NS - 2)>();
         __syncthreads();
         clean(0);
@@ -1243,6 +1313,11 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         }
         // nothing may still be on its way to LDS when the workgroup ends
         wait_loads<0>();
+    } else if (prefix) {
+        // the page table does not reach that far
+        prefix_limits<ROWS>(a, wk, sh.limit);
+#pragma unroll
+        for (int n = 0; n != NT; ++n) set_limit(a, wk, sh.limit, row[n]);
     }
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
@@ -1274,36 +1349,37 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
 }
 
-// Sixteen lanes per row: the references and sums of its cuts decide their weights, then the cuts'
-// O are added in order.
-template <typename T, int D>
+// The references and sums of a row's cuts decide their weights, then the cuts' O are added in a
+// fixed order: TEAMS teams of sixteen lanes per row take them in turn (four teams where many cuts
+// are to be joined, one where many rows are).
+template <typename T, int D, int TEAMS>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t a)
 {
     constexpr int LANES = 16, PER = D / LANES;
     int const     lane = int(threadIdx.x) % LANES;
+    int const     team = int(threadIdx.x) / LANES % TEAMS;
     int const     heads = a.h_kv * a.group;
-    int const     id = int(blockIdx.x) * (THREADS / LANES) + int(threadIdx.x) / LANES;
+    int const     id = int(blockIdx.x) * (THREADS / LANES / TEAMS) +
+                   int(threadIdx.x) / (LANES * TEAMS);
     int const     token = id / heads, head = id - token * heads;
     if (token >= a.n_tokens) return;
-    int const* const meta = a.part_meta + 4 * token;
-    int const        from = meta[0], said = meta[1], b = meta[2];
-    if (token < a.offsets[0] || token >= a.offsets[a.n_seqs]) return;
-    int const splits = min(said, a.items);
-    if (splits <= 0) return;
     int const kvh = head / a.group, hg = head - kvh * a.group;
-    int const prow = token * a.group + hg, srow = (token - b) * a.group + hg;
+    int const prow = token * a.group + hg;
+    int4 const meta = a.part_meta[prow];
+    if (token < a.offsets[0] || token >= a.offsets[a.n_seqs]) return;
+    if (meta.y < 0) return;  // stored already
+    // both stay inside the workspace whatever the device arrays held
+    int const whole = min(meta.y, a.own_slots), srow = min(max(meta.w, 0), a.own_rows - 1);
     int const pslot = a.prefix_splits ? prow / a.prefix_rows : 0;
-    int const sslot = from + srow / a.own_rows * splits;
-    int const parts = a.prefix_splits + splits;
+    int const parts = a.prefix_splits + whole + (meta.z >= 0);
     auto      place = [&](int i) -> int64_t {
         if (i < a.prefix_splits) {
             return (int64_t(pslot + i * a.prefix_tiles) * a.h_kv + kvh) * a.prefix_rows +
                    prow % a.prefix_rows;
         }
-        // stays inside the workspace whatever the device arrays held
-        int const slot = min(max(sslot + i - a.prefix_splits, 0), a.items - 1);
-        return a.own_base + (int64_t(slot) * a.h_kv + kvh) * a.own_rows +
-               max(srow, 0) % a.own_rows;
+        i -= a.prefix_splits;
+        int const slot = min(max(i < whole ? meta.x + i : meta.z, 0), a.own_slots - 1);
+        return a.own_base + (int64_t(slot) * a.h_kv + kvh) * a.own_rows + srow;
     };
     float top = NEG_INF;
     for (int i = lane; i < parts; i += LANES) top = fmaxf(top, a.part_ml[place(i) * 2]);
@@ -1324,15 +1400,15 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
         sum += mi == NEG_INF ? 0.0f : li * f;
         constexpr int U = 4;  // cuts in flight
         int const     n = min(parts - i0, LANES);
-        for (int i = 0; i < n; i += U) {
+        for (int i = team; i < n; i += U * TEAMS) {
             float4_t x[U][PER / 4];
             float    fi[U];
 #pragma unroll
             for (int u = 0; u != U; ++u) {
-                int const     which = group0 + min(i + u, n - 1);
+                int const     which = group0 + min(i + u * TEAMS, n - 1);
                 int64_t const p = __shfl(at, which);
                 float const   fu = __shfl(f, which);
-                fi[u] = i + u < n ? fu : 0.0f;
+                fi[u] = i + u * TEAMS < n ? fu : 0.0f;
                 // a cut without weight may hold anything
                 float4_t const* const src =
                     reinterpret_cast<float4_t const*>(a.part_o + p * D + lane * PER);
@@ -1350,6 +1426,15 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
     }
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor(sum, o);
+#pragma unroll
+    for (int o = LANES; o < LANES * TEAMS; o <<= 1) {
+#pragma unroll
+        for (int e = 0; e != PER / 4; ++e) {
+#pragma unroll
+            for (int i = 0; i != 4; ++i) y[e][i] += __shfl_xor(y[e][i], o);
+        }
+    }
+    if (team != 0) return;
     T* const    dst = reinterpret_cast<T*>(a.out) + uint64_t(token) * a.out_stride +
                    uint64_t(head) * uint64_t(a.d) + lane * PER;
     float const inv = top == NEG_INF ? 0.0f : 1.0f / sum;
@@ -1376,7 +1461,7 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
 {
     a.parts = parts;
     uint64_t const units = (parts & 1 ? uint64_t(a.prefix_tiles) * a.prefix_splits : 0) +
-                           (parts & 2 ? a.items : 0);
+                           (parts & 2 ? a.own_slots : 0);
     uint32_t const grid = uint32_t((units + 7) / 8 * 8 * a.h_kv);
     if constexpr (sizeof(T) == 2) {
         if constexpr (D <= 128) {
@@ -1414,9 +1499,15 @@ void launch_dim(attention_dev_t const& a, hipStream_t stream)
         if (a.prefix_splits != 0) launch_rows<T, D>(a, 1, a.prefix_rows, stream);
         launch_rows<T, D>(a, 2, a.own_rows, stream);
     }
-    if (a.prefix_splits != 0 || a.split_target != 0) {
+    if (a.prefix_splits != 0 || a.shares != 0) {
         uint64_t const rows = uint64_t(a.n_tokens) * a.h_kv * a.group;
-        attention_join_kernel<T, D><<<uint32_t((rows + 15) / 16), THREADS, 0, stream>>>(a);
+        if (a.prefix_splits >= 8 || rows <= 4096) {
+            attention_join_kernel<T, D, 4>
+                <<<uint32_t((rows + 3) / 4), THREADS, 0, stream>>>(a);
+        } else {
+            attention_join_kernel<T, D, 1>
+                <<<uint32_t((rows + 15) / 16), THREADS, 0, stream>>>(a);
+        }
     }
 }
 
@@ -1460,8 +1551,8 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (shared > 0) {
         p.prefix_rows = tile_rows(c, rows);
         uint64_t const tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
-        uint64_t W = 512; if (getenv("X_PRE")) W = atoi(getenv("X_PRE"));
-        uint64_t const want = (W + tiles * kv - 1) / (tiles * kv);
+        uint64_t const slots = p.prefix_rows == FEW ? 1024 : 256;
+        uint64_t const want = (slots + tiles * kv - 1) / (tiles * kv);
         uint64_t const most = (shared + 255) / 256;
         uint64_t const splits = std::max<uint64_t>(1, std::min(want, most));
         uint64_t const chunk = ((shared + splits - 1) / splits + 63) / 64 * 64;
@@ -1477,16 +1568,13 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (2 * group <= p.own_rows + 1) {
         tiles = std::min(tiles, seqs + (rows - seqs * group) / (p.own_rows - group + 1));
     }
-    uint64_t fill = 1024 / kv;
-    if (getenv("X_FILL")) fill = atoi(getenv("X_FILL")) / kv;
-    uint64_t const target =
-        tiles * kv >= 8192 ? 0 : std::max(fill > tiles ? fill - tiles : 0, (tiles + 1) / 2);
-    p.split_target = uint32_t(target);
-    p.items = uint32_t(tiles + target);
-    part_rows += p.items * kv * p.own_rows;
+    uint64_t const aim = p.own_rows == FEW ? 1024 : 512;
+    p.shares = tiles * kv >= 4 * aim ? 0 : uint32_t(std::max<uint64_t>(1, aim / kv));
+    p.own_slots = uint32_t(tiles + p.shares);
+    part_rows += p.own_slots * kv * p.own_rows;
     p.part_rows = part_rows;
     p.workspace_bytes = up256(part_rows * uint64_t(padded_dim(c.head_dim)) * 4) +
-                        up256(part_rows * 8) + up256(uint64_t(n_tokens) * 16);
+                        up256(part_rows * 8) + up256(rows * 16);
     return p;
 }
 
@@ -1529,8 +1617,12 @@ void launch_attention(attention_args_t const& g, attention_plan_t const& p, void
     a.prefix_splits = int(p.prefix_splits);
     a.prefix_chunk = int(p.prefix_chunk);
     a.prefix_rows = int(p.prefix_rows);
-    a.split_target = int(p.split_target);
-    a.items = int(p.items);
+    a.shares = int(p.shares);
+    a.own_slots = int(p.own_slots);
+    // the units of the whole batch are counted in 32 bits
+    uint64_t const reach = uint64_t(a.max_pages) * uint64_t(a.page_size) / 16 + 2;
+    a.grain = 1;
+    while (uint64_t(p.own_slots) * (reach / uint64_t(a.grain) + 1) >= (1ull << 30)) a.grain *= 2;
     a.own_rows = int(p.own_rows);
     a.own_base = int64_t(p.own_base);
     a.direct = p.prefix_splits == 0;
@@ -1539,7 +1631,7 @@ void launch_attention(attention_args_t const& g, attention_plan_t const& p, void
     uint64_t const o_bytes = up256(p.part_rows * uint64_t(padded_dim(a.d)) * 4);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + o_bytes);
-    a.part_meta = reinterpret_cast<int*>(ws + o_bytes + up256(p.part_rows * 8));
+    a.part_meta = reinterpret_cast<int4*>(ws + o_bytes + up256(p.part_rows * 8));
     if (g.cache.dtype == ES_KM_F16) {
         launch_type<_Float16>(a, stream);
     } else {

@@ -64,8 +64,8 @@ struct attention_plan_t {
     uint32_t prefix_splits = 0;  // cuts of the shared positions
     uint32_t prefix_chunk = 0;   // positions per cut
     uint32_t own_rows = 0;       // rows per tile, the sequences' own positions
-    uint32_t split_target = 0;   // cuts of the own positions, over the whole batch
-    uint32_t items = 0;          // upper bound of (row tile, cut) pairs of the own positions
+    uint32_t shares = 0;         // parts of the own positions of the whole batch
+    uint32_t own_slots = 0;      // upper bound of (row tile, part) pairs of the own positions
     uint64_t own_base = 0;       // rows of partial results before the own positions'
     uint64_t part_rows = 0;      // rows of partial results
     uint64_t workspace_bytes = 0;
