@@ -172,13 +172,13 @@ __device__ inline void set_limit(attention_dev_t const& a, work_t const& k, int 
     }
 }
 
-// Workgroups go to the eight XCDs in turn.  The heads of one unit (a row tile and a cut) stay on
-// one XCD: together they read whole rows of the cache.
+// Workgroups go to the eight XCDs in turn, so with the key heads innermost every XCD gets the same
+// heads of all units: equal work however long the sequences are, and tiles that read the same keys
+// share an L2.
 __device__ inline void unit_of_block(attention_dev_t const& a, int& unit, int& kvh)
 {
-    int const xcd = int(blockIdx.x) & 7, i = int(blockIdx.x) >> 3;
-    kvh = i % a.h_kv;
-    unit = i / a.h_kv * 8 + xcd;
+    kvh = int(blockIdx.x) % a.h_kv;
+    unit = int(blockIdx.x) / a.h_kv;
 }
 
 // A prefix workgroup: a tile of the batch's rows against a cut of the shared positions.
@@ -681,7 +681,7 @@ struct few_shared_t {
     static constexpr int DJ = D < 128 ? D : 128;  // elements joined at a time
     deal_t  deal;
     int     limit[FEW];
-    int64_t off[WAVES][2][16];
+    int64_t off[WAVES][16];
     float   m[WAVES][FEW], l[WAVES][FEW];
     union {
         float                          o[WAVES][FEW][DJ + 4];
@@ -691,7 +691,7 @@ struct few_shared_t {
 
 // The workgroup's keys against the tile's rows; steps w, w + WAVES, ...
 template <typename T, int D, bool PAD>
-__device__ void attend_few(attention_dev_t const& a, int64_t (*offs)[16],
+__device__ void attend_few(attention_dev_t const& a, int64_t* off,
                            typename core_t<T, D>::query_t const (*q)[64], work_t const& wk,
                            row_t const& row, int least, int kvh, float4_t* o, float& m, float& l)
 {
@@ -706,52 +706,39 @@ __device__ void attend_few(attention_dev_t const& a, int64_t (*offs)[16],
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
-    // two steps ahead: the page of this lane's key (-1: not among them, or no such page)
+    // A step ahead: the page of this lane's key.  Positions that are not the workgroup's stand for
+    // its first or last.
     int  page = -1, prow = 0;
     auto look_up = [&](int at) {
-        int const pos = at + (lane & (KS - 1));
-        page = -1;
-        if (pos >= lo && pos < hi) {
-            int const pi = page_of(a, pos);
-            prow = pos - pi * a.page_size;
-            page = wk.table[pi];
-        }
-    };
-    // where the looked-up keys lie, for all lanes; true: some are nowhere
-    auto place = [&](int64_t* off) {
-        int64_t const at = entry_of(a, page, prow);
-        __builtin_amdgcn_wave_barrier();
-        if (lane < KS) off[lane] = at;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        return bool(__any(at < 0));
+        int const pos = min(max(at + (lane & (KS - 1)), lo), hi - 1);
+        int const pi = page_of(a, pos);
+        prow = pos - pi * a.page_size;
+        page = wk.table[pi];
     };
     constexpr int STEP = WAVES * KS;
     int           base = (lo / KS + w) * KS;
     float         ref = 0;
     bool          bad = false;
     look_up(base);
-    bool holes = place(offs[0]), holes_next = false;
-    look_up(base + STEP);
-    x.template load_k<PAD>(kb, offs[0], c, g, a.d);
-    x.template load_v<PAD>(vb, offs[0], c, g, a.d);
-    // The next step's K is asked for as soon as this step's scores are computed, its V after this
-    // step's values: a wavefront always has one of the two on its way.  Behind the last step, too
-    // (positions that are not there read the cache's first entry): loads under a condition made
-    // the compiler take registers of V for free.
-    for (int turn = 0; base < hi; base += STEP, turn ^= 1) {
-        int64_t const* const off = offs[turn];
-        holes_next = place(offs[turn ^ 1]);
-        look_up(base + 2 * STEP);
+    for (; base < hi; base += STEP) {
+        // where the keys lie, for all lanes; -1: no such page
+        int64_t const at = entry_of(a, page, prow);
+        bool const    holes = __any(at < 0);
+        __builtin_amdgcn_wave_barrier();
+        if (lane < KS) off[lane] = at;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        x.template load_k<PAD>(kb, off, c, g, a.d);
+        x.template load_v<PAD>(vb, off, c, g, a.d);
+        look_up(base + STEP);
+        // all of the step's loads go out before the first is waited for; what hides their latency
+        // is the other fifteen wavefronts of the compute unit
         __builtin_amdgcn_sched_barrier(0);
         x.template trim_k<PAD>(g, a.d);
         float s[KL];
         x.scores(s, q, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        x.template load_k<PAD>(kb, offs[turn ^ 1], c, g, a.d);
-        __builtin_amdgcn_sched_barrier(0);
         x.template trim_v<PAD>(c, a.d);
-        bool const edge = holes || base + KS - 1 > seen_by_all;
+        bool const edge = holes || base < lo || base + KS > hi || base + KS - 1 > seen_by_all;
         uint32_t   masked = 0;
         if (edge) {
 #pragma unroll
@@ -762,7 +749,8 @@ __device__ void attend_few(attention_dev_t const& a, int64_t (*offs)[16],
                 // added in the end to the rows that see them
                 x.keep_key(j, !hole);
                 bad |= x.clean_key(j);
-                masked |= hole || base + key > row.limit ? 1u << j : 0;
+                masked |= hole || base + key < lo || base + key > min(hi - 1, row.limit) ? 1u << j
+                                                                                        : 0;
             }
         }
         float top = NEG_INF;
@@ -780,9 +768,6 @@ __device__ void attend_few(attention_dev_t const& a, int64_t (*offs)[16],
         }
         l += sum;
         x.values(s, o);
-        __builtin_amdgcn_sched_barrier(0);
-        x.template load_v<PAD>(vb, offs[turn ^ 1], c, g, a.d);
-        holes = holes_next;
     }
     if (__any(bad)) {
         for (base = (lo / KS + w) * KS; base < hi; base += STEP) {
@@ -918,7 +903,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 2 : D == 128 && sizeof(T) == 4 
 
 // ------------------------------------------------------------------------------ many rows
 
-// What rows without an entry, and elements beyond head_dim, are loaded from.
+// What positions without a page, and elements beyond head_dim, are loaded from.
 __device__ __align__(16) uint32_t const attention_zeros[128] = {0};
 
 // 64 lanes x 16 bytes from each lane's address to LDS at lds + 16 * lane.
@@ -1012,9 +997,10 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
 
     // this thread's position of window n, and its page number
     auto position = [&](int n) { return first + n * M::WINDOW + tid; };
-    auto page_at = [&](int pos) {
-        return wk.table + (pos >= lo && pos < hi ? page_of(a, pos) : page_of(a, lo));
-    };
+    // (positions that are not the workgroup's stand for its first or last: one place for all of
+    // them would be a hot spot in the caches)
+    auto inside = [&](int pos) { return min(max(pos, lo), hi - 1); };
+    auto page_at = [&](int pos) { return wk.table + page_of(a, inside(pos)); };
     int page0 = -1;
     if (lo < hi) page0 = *page_at(position(0));
 
@@ -1051,12 +1037,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         int               least = 0x7fffffff, most = -1;
 
         auto put_entry = [&](int n, int page) {
-            int const pos = position(n);
-            int64_t   at = -1;
-            if (pos >= lo && pos < hi) {
-                at = entry_of(a, page, pos - page_of(a, pos) * a.page_size);
-                if (at < 0) sh.holes = 1;
-            }
+            int const     pos = inside(position(n));
+            int64_t const at = entry_of(a, page, pos - page_of(a, pos) * a.page_size);
+            if (at < 0) sh.holes = 1;
             sh.kat[n & 1][tid] = at < 0 ? zeros : kb + at * 2;
             sh.vat[n & 1][tid] = at < 0 ? zeros : vb + at * 2;
         };
@@ -1121,11 +1104,11 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             for (int t = 0; t != ST; ++t) {
 #pragma unroll
                 for (int r = 0; r != 4; ++r) {
-                    int const  key = 16 * t + 4 * g + r;
-                    bool const none = at[key] == zeros;  // not among the positions, or no page
+                    int const  key = 16 * t + 4 * g + r, pos = base + key;
+                    bool const none = pos < lo || pos >= hi || at[key] == zeros;  // no page
 #pragma unroll
                     for (int n = 0; n != NT; ++n) {
-                        if (none || base + key > row[n].limit) s[n][t][r] = NEG_INF;
+                        if (none || pos > row[n].limit) s[n][t][r] = NEG_INF;
                     }
                 }
             }
@@ -1153,7 +1136,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         put_entry(0, page0);
         __syncthreads();
         load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
-        // beyond the last tile too: the waits count instructions (the entries are zeros)
+        // beyond the last tile too: the waits count instructions
 #pragma unroll
         for (int i = 0; i != NS - 1; ++i) {
             aim(i);
@@ -1462,7 +1445,7 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
     a.parts = parts;
     uint64_t const units = (parts & 1 ? uint64_t(a.prefix_tiles) * a.prefix_splits : 0) +
                            (parts & 2 ? a.own_slots : 0);
-    uint32_t const grid = uint32_t((units + 7) / 8 * 8 * a.h_kv);
+    uint32_t const grid = uint32_t(units * a.h_kv);
     if constexpr (sizeof(T) == 2) {
         if constexpr (D <= 128) {
             if (rows == many_t<D, 2>::ROWS) {
