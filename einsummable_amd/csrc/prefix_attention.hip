@@ -1229,7 +1229,6 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                     }
                 }
             }
-            if (edge(tile + 1)) mask(tile + 1, next);
             // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of its
             // own element
             typedef short tr_t __attribute__((ext_vector_type(4)));
@@ -1264,6 +1263,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                         __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[n][ks], o[n][DT], 0, 0, 0);
                 }
             }
+            // (last: a branch between the scores and the values would keep them from overlapping)
+            if (edge(tile + 1)) mask(tile + 1, next);
             raise_all(next);
         };
         for (int tile = 0; tile < tiles; tile += NS) {
