@@ -10,13 +10,18 @@ attention scale 1/sqrt(head_dim) is computed but not applied (modules.cc:323-344
 
 Buffers are named byte ranges; a node reads and writes them under its own dtype (the
 "complexer" view of an f32 tensor as c64 is the same bytes under another name).
+
+LayerGraph computes whole sequences at once.  DecodeGraph is the same layer for tokens that
+continue sequences: keys and values live in a paged cache, and the serving operators take the
+place of the rotation, the attention's nodes and, with 4-bit weights, the linear products.
 """
 import math
 
-from .km import C64, F16, F32, Einsummable, Touch
+from .km import C64, F16, F32, ROPE_PAIRS, Einsummable, Int4Weight, KvBatch, KvCache, Touch
 
+U8, I32 = "u8", "i32"   # dtypes of inputs only, no einsummable's
 DT_NAME = {F16: "f16", F32: "f32", C64: "c64"}
-DT_SIZE = {F16: 2, F32: 4, C64: 8}
+DT_SIZE = {F16: 2, F32: 4, C64: 8, U8: 1, I32: 4}
 
 
 def _g6(v):
@@ -166,11 +171,16 @@ class LayerGraph:
         h1 = self.es("residual1", Einsummable([s * d], [[0], [0]], 1, add),
                      self.buf("residual1", F16, s * d), [x, ao])
 
-        # feed forward: w2(silu(w1 x) * w3 x)
+        self.feed_forward(h1, w_fn, w1, w2, w3)
+
+    def feed_forward(self, h1, w_fn, w1, w2, w3):
+        """w2(silu(w1 x) * w3 x) behind a residual"""
+        s, d, f = self.seq, self.dim, self.ffn
         xf = self.rms_norm("fn.", h1, w_fn)
         a1 = self.linear("w1", xf, w1, d, f)
         a3 = self.linear("w3", xf, w3, d, f)
         silu = "*[hole|f16@0,power{-1}[+[constant{f16|1},exp[*[constant{f16|-1},hole|f16@0]]]]]"
+        mul, add = "*[hole|f16@0,hole|f16@1]", "+[hole|f16@0,hole|f16@1]"
         g = self.unary("silu", silu, a1, F16, F16, s * f)
         g = self.es("gate", Einsummable([s * f], [[0], [0]], 1, mul), self.buf("gate", F16, s * f),
                     [g, a3])
@@ -180,6 +190,94 @@ class LayerGraph:
 
     def contraction_flops(self):
         return sum(n.get("flops", 0) for n in self.nodes)
+
+
+class DecodeGraph(LayerGraph):
+    """The decoder layer for n_tokens new tokens of n_seqs sequences over a paged cache of keys and
+    values.
+
+    Inputs besides x and the norms' weights: cache.k and cache.v ([page, position, head, element];
+    the append node writes into them), offsets, lens and page_table (int32, as es_km_kv_batch_t
+    has them), full_freqs_cis.  A captured graph sees what they hold at replay.  The first `shared`
+    positions are a prefix that all sequences have in common.
+    int4_group: None for f16 weights [n_out, n_in], else the group of 4-bit ones, w.q, w.scales
+    and w.zeros for each weight w (quantize_int4).
+    scale: the reference computes 1/sqrt(head_dim) and leaves it out (modules.cc:323-344)."""
+
+    def __init__(self, n_tokens, n_seqs, n_pages, page_size, max_pages, n_pos, shared=0, dim=4096,
+                 n_heads=32, n_kv_heads=None, ffn=11008, int4_group=None, scale=1.0, eps=1e-6):
+        self.n_seqs, self.n_pages, self.page_size = n_seqs, n_pages, page_size
+        self.max_pages, self.n_pos, self.shared, self.scale = max_pages, n_pos, shared, scale
+        self.n_kv, self.int4_group = n_kv_heads or n_heads, int4_group
+        assert n_heads % self.n_kv == 0
+        super().__init__(dim, n_heads, ffn, n_tokens, eps)
+
+    def weight(self, name, n_out, n_in):
+        if self.int4_group is None:
+            return self.inp(name, F16, (n_out, n_in))
+        groups = -(-n_in // self.int4_group)
+        return (self.inp(name + ".q", U8, (n_out, n_in // 2)),
+                self.inp(name + ".scales", F16, (n_out, groups)),
+                self.inp(name + ".zeros", U8, (n_out, groups)))
+
+    def linear(self, label, x, w, n_in, n_out):
+        if self.int4_group is None:
+            return super().linear(label, x, w, n_in, n_out)
+        y = self.buf(label + ".mm", F16, self.seq * n_out)
+        self.nodes.append({"kind": "int4_linear", "label": label, "out": y, "inn": x, "w": w,
+                           "shape": (self.seq, n_out, n_in), "group": self.int4_group})
+        return y
+
+    def _build(self):
+        s, d, h, hd, f = self.seq, self.dim, self.n_heads, self.hd, self.ffn
+        kv = self.n_kv * hd
+        x = self.inp("x", F16, (s, d))
+        w_an = self.inp("attention_norm.weight", F16, (d,))
+        wq, wo = self.weight("wq", d, d), self.weight("wo", d, d)
+        wk, wv = self.weight("wk", kv, d), self.weight("wv", kv, d)
+        w_fn = self.inp("ffn_norm.weight", F16, (d,))
+        w1, w3 = self.weight("w1", f, d), self.weight("w3", f, d)
+        w2 = self.weight("w2", d, f)
+        freqs = self.inp("full_freqs_cis", C64, (self.n_pos, hd // 2))
+        pages = (self.n_pages, self.page_size, self.n_kv, hd)
+        cache = (self.inp("cache.k", F16, pages), self.inp("cache.v", F16, pages))
+        batch = (self.inp("offsets", I32, (self.n_seqs + 1,)), self.inp("lens", I32, (self.n_seqs,)),
+                 self.inp("page_table", I32, (self.n_seqs, self.max_pages)))
+
+        xa = self.rms_norm("an.", x, w_an)
+        q = self.linear("wq", xa, wq, d, d)
+        k = self.linear("wk", xa, wk, d, kv)
+        v = self.linear("wv", xa, wv, d, kv)
+        rot = self.buf("q.rotated", F16, s * d)
+        self.nodes.append({"kind": "kv_append", "label": "append", "out": rot, "inns": [q, k, v],
+                           "cache": cache, "batch": batch, "freqs": freqs})
+        at = self.buf("values", F16, s * d)
+        self.nodes.append({"kind": "prefix_attention", "label": "attention", "out": at, "inn": rot,
+                           "cache": cache, "batch": batch})
+        ao = self.linear("wo", at, wo, d, d)
+        add = "+[hole|f16@0,hole|f16@1]"
+        h1 = self.es("residual1", Einsummable([s * d], [[0], [0]], 1, add),
+                     self.buf("residual1", F16, s * d), [x, ao])
+        self.feed_forward(h1, w_fn, w1, w2, w3)
+
+
+def quantize_int4(w, group):
+    """(q, scales, zeros) of a weight [n, k] for Int4Weight: per row and group the 16 steps from
+    its least to its largest value (zero among them)."""
+    import numpy as np
+
+    n, k = w.shape
+    groups = -(-k // group)
+    wide = np.zeros((n, groups * group), np.float32)
+    wide[:, :k] = w
+    wide = wide.reshape(n, groups, group)
+    lo, hi = np.minimum(wide.min(-1), 0), np.maximum(wide.max(-1), 0)
+    # the steps as the kernel will see them; a step that f16 has not got would divide by zero
+    scales = np.maximum((hi - lo) / 15, np.float32(2.0 ** -24)).astype(np.float16)
+    zeros = np.clip(np.rint(-lo / scales), 0, 15)
+    q = np.clip(np.rint(wide / scales[..., None].astype(np.float32)) + zeros[..., None], 0, 15)
+    q = q.reshape(n, -1)[:, :k].astype(np.uint8)
+    return q[:, 0::2] | (q[:, 1::2] << 4), scales, zeros.astype(np.uint8)
 
 
 def freqs_cis_table(n_pos, half_dim, theta=10000.0):
@@ -197,21 +295,53 @@ class DeviceRunner:
     """Owns one device buffer per named range (a stand-in for the engine's arena) and runs the
     node list in order on one stream.  Every node goes through the C ABI."""
 
-    def __init__(self, km, graph):
+    def __init__(self, km, graph, mem=None):
+        """`mem`: buffers (uint8 tensors, by name) to use instead of own ones, such as another
+        runner's weights and cache; runners that share a cache run one after the other."""
         import torch
 
         self.km, self.g, self.torch = km, graph, torch
-        self.mem = {name: torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-                    for name, nbytes in graph.buffers.items()}
+        self.mem = dict(mem or {})
+        for name, nbytes in graph.buffers.items():
+            if name not in self.mem:
+                self.mem[name] = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+            assert self.mem[name].numel() == nbytes, name
         need = 0
         for n in graph.nodes:
             if n["kind"] == "einsummable":
                 ws = km.build(n["e"])
                 assert ws is not None, "no kernel for node " + n["label"]
-                n["ws"] = ws
-                need = max(need, ws)
+            elif n["kind"] in ("kv_append", "prefix_attention", "int4_linear"):
+                ws = self._serving(n)
+            else:
+                continue
+            n["ws"] = ws
+            need = max(need, ws)
         # one scratch buffer serves every node: they run one after the other on one stream
         self.workspace = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+
+    def _serving(self, n):
+        """Descriptors of a serving node and its call; returns the workspace it needs."""
+        km, g = self.km, self.g
+        at = {name: m.data_ptr() for name, m in self.mem.items()}
+        if n["kind"] == "int4_linear":
+            m, n_out, n_in = n["shape"]
+            q, scales, zeros = n["w"]
+            w = Int4Weight(F16, n_out, n_in, n["group"], at[q], at[scales], at[zeros])
+            n["call"] = lambda stream, ws: km.int4_linear(w, m, stream, at[n["out"]], at[n["inn"]],
+                                                          ws)
+            return km.int4_linear_workspace(w, m)
+        cache = KvCache(F16, g.n_heads, g.n_kv, g.hd, g.n_pages, g.page_size,
+                        *[at[c] for c in n["cache"]])
+        batch = KvBatch(g.n_seqs, g.seq, *[at[b] for b in n["batch"]], g.max_pages)
+        if n["kind"] == "kv_append":
+            n["call"] = lambda stream, ws: km.kv_append(cache, batch, stream, at[n["out"]],
+                                                        *[at[b] for b in n["inns"]], ROPE_PAIRS,
+                                                        at[n["freqs"]], g.n_pos)
+            return 0
+        n["call"] = lambda stream, ws: km.prefix_attention(cache, batch, g.shared, g.scale, stream,
+                                                           at[n["out"]], at[n["inn"]], ws)
+        return km.prefix_attention_workspace(cache, g.n_seqs, g.seq, g.shared)
 
     def set_input(self, name, array):
         import numpy as np
@@ -237,6 +367,8 @@ class DeviceRunner:
                 elif n["kind"] == "touch":
                     km.touch(n["t"], stream, self.mem[n["out"]].data_ptr(),
                              self.mem[n["inn"]].data_ptr())
+                elif "call" in n:
+                    n["call"](stream, (self.workspace.data_ptr(), n["ws"]) if n["ws"] else None)
                 else:
                     assert n["dtype"] == F16
                     lo = struct.unpack("<H", struct.pack("<e", n["lower"]))[0]
@@ -298,6 +430,8 @@ class ArenaRunner:
                                        [self.ranges[b] for b in n["inns"]])
             elif n["kind"] == "touch":
                 i = ag.add_touch(n["t"], -1, [self.ranges[n["out"]], self.ranges[n["inn"]]])
+            elif n["kind"] != "lowertri":
+                raise NotImplementedError("the exec graph has no %s nodes" % n["kind"])
             else:
                 assert n["dtype"] == F16
                 lo = struct.unpack("<H", struct.pack("<e", n["lower"]))[0]
