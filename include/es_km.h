@@ -274,7 +274,7 @@ int es_km_prefix_attention(es_km_t* km, const es_km_kv_cache_t* cache,
  * w_stride bytes from row to row; scales: the dtype of x and y; zeros: uint8, or NULL for 8
  * everywhere; both ceil(k / group) to a row, rows scale_stride apart.  k and group are
  * multiples of 32, group at least 32; x and w (bases and strides) sit on 16-byte boundaries.
- * Meant for few tokens (m): the weight is streamed once per 64 of them (f16; 16 in f32).
+ * Meant for few tokens (m): the weight is streamed once per 64 of them (f16; 21 in f32).
  * Products of integers and activations are exact, sums fp32.  f32 activations are split into
  * three f16 parts relative to their row's largest magnitude (33 bits in all) in the
  * workspace, whose size es_km_int4_linear_workspace reports (0 for f16). */

@@ -10,6 +10,9 @@
 //   operator()(touch_t, stream, out, inn)
 //   constant_fill / lowerTri_fill
 //
+// and, beside the reference's members, the serving operators over a paged cache: kv_append,
+// prefix_attention, int4_linear, each with the workspace it needs.
+//
 // The descriptor structs carry the same fields as the reference's einsummable_t
 // (src/einsummable/einsummable.h:8-20), touch_t (touch.h:8-29) and fill_t (fill.h:11-30); the
 // join travels as the text `operator<<(ostream&, scalarop_t)` writes.  Inside the reference
@@ -201,6 +204,51 @@ public:
         uint64_t n = 1;
         for (uint64_t d : c.shape) n *= d;
         check(es_km_fill_constant(h_, int(c.value.dtype), c.value.bits(), n, stream, out));
+    }
+
+    // es_km_kv_append; strides in elements from token to token.  q and q_out may both be null.
+    void kv_append(es_km_kv_cache_t const& cache, es_km_kv_batch_t const& batch, void* stream,
+                   void* q_out, void const* q, void const* k, void const* v,
+                   uint64_t q_out_stride, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                   int rope = ES_KM_ROPE_NONE, void const* freqs = nullptr,
+                   uint64_t n_pos = 0) const
+    {
+        check(es_km_kv_append(h_, &cache, &batch, stream, q_out, q, k, v, q_out_stride, q_stride,
+                              k_stride, v_stride, rope, freqs, n_pos));
+    }
+
+    // es_km_prefix_attention; the first `shared` positions are the same for every sequence.
+    uint64_t prefix_attention_workspace(es_km_kv_cache_t const& cache, int n_seqs, int n_tokens,
+                                        uint64_t shared) const
+    {
+        uint64_t ws = 0;
+        check(es_km_prefix_attention_workspace(h_, &cache, n_seqs, n_tokens, shared, &ws));
+        return ws;
+    }
+    void prefix_attention(es_km_kv_cache_t const& cache, es_km_kv_batch_t const& batch,
+                          uint64_t shared, float scale, void* stream, void* out, void const* q,
+                          uint64_t out_stride, uint64_t q_stride,
+                          std::optional<std::tuple<void*, uint64_t>> workspace = std::nullopt) const
+    {
+        check(es_km_prefix_attention(h_, &cache, &batch, shared, scale, stream, out, q, out_stride,
+                                     q_stride, workspace ? std::get<0>(workspace.value()) : nullptr,
+                                     workspace ? std::get<1>(workspace.value()) : 0));
+    }
+
+    // es_km_int4_linear: y = x W^T for m tokens.
+    uint64_t int4_linear_workspace(es_km_int4_weight_t const& weight, uint64_t m) const
+    {
+        uint64_t ws = 0;
+        check(es_km_int4_linear_workspace(h_, &weight, m, &ws));
+        return ws;
+    }
+    void int4_linear(es_km_int4_weight_t const& weight, uint64_t m, void* stream, void* y,
+                     void const* x, uint64_t y_stride, uint64_t x_stride,
+                     std::optional<std::tuple<void*, uint64_t>> workspace = std::nullopt) const
+    {
+        check(es_km_int4_linear(h_, &weight, m, stream, y, x, y_stride, x_stride,
+                                workspace ? std::get<0>(workspace.value()) : nullptr,
+                                workspace ? std::get<1>(workspace.value()) : 0));
     }
 
 private:

@@ -1,10 +1,15 @@
 """The serving operators' checks of their arguments, which need no device: without a handle a call
 gets its checks and, when they all pass, "null handle".  No pointer below is ever followed."""
 import ctypes
+import os
+import subprocess
 
+import numpy as np
 import pytest
 
 import einsummable_amd as ea
+from einsummable_amd.llama_layer import DecodeGraph, quantize_int4
+from serving_oracle import int4_pack
 
 OK, UNSUPPORTED, INVALID, WORKSPACE = 0, 1, -1, -3
 A = 1 << 20   # an address on a 256-byte boundary
@@ -171,3 +176,64 @@ def test_workspaces():
         assert ws.value >= tokens * 8 * 64 * 4
         sizes.append(ws.value)
     assert sizes == sorted(sizes)
+
+
+# ------------------------------------------------------------------------------ C++ and the layer
+
+def test_cxx_members_compile(tmp_path):
+    """The header's members take what the C entries take."""
+    src = tmp_path / "serving.cc"
+    src.write_text("""
+#include "es_km.hpp"
+void step(eskm::kernel_manager_t const& km, es_km_kv_cache_t const& c, es_km_kv_batch_t const& b,
+          es_km_int4_weight_t const& w, void* p)
+{
+    km.kv_append(c, b, nullptr, p, p, p, p, 8, 8, 8, 8);
+    km.kv_append(c, b, nullptr, nullptr, nullptr, p, p, 0, 0, 8, 8, ES_KM_ROPE_PAIRS, p, 16);
+    uint64_t const n = km.prefix_attention_workspace(c, 1, 1, 64);
+    km.prefix_attention(c, b, 64, 0.5f, nullptr, p, p, 8, 8, std::make_tuple(p, n));
+    km.prefix_attention(c, b, 0, 0.5f, nullptr, p, p, 8, 8);
+    uint64_t const m = km.int4_linear_workspace(w, 1);
+    km.int4_linear(w, 1, nullptr, p, p, 8, 32, std::make_tuple(p, m));
+    km.int4_linear(w, 1, nullptr, p, p, 8, 32);
+}
+""")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["g++", "-std=c++17", "-fsyntax-only", "-Wall", "-Werror", "-I", include,
+                    str(src)], check=True)
+
+
+@pytest.mark.parametrize("k,group", [(64, 32), (160, 64), (96, 128)])
+def test_quantize_int4(k, group):
+    """Within half a step of the weight (and what rounding the step to f16 moves the 15 steps:
+    15 * 2^-11), zero kept exactly, ranges without zero and empty ones included."""
+    r = np.random.RandomState(k)
+    w = r.normal(0, 1, (6, k)).astype(np.float32)
+    w[1] = np.abs(w[1]) + 1
+    w[2] = -np.abs(w[2])
+    w[3] = 0
+    w[4, ::3] = 0
+    packed, scales, zeros = quantize_int4(w, group)
+    assert packed.dtype == zeros.dtype == np.uint8 and scales.dtype == np.float16
+    assert packed.shape == (6, k // 2) and scales.shape == zeros.shape == (6, -(-k // group))
+    q = np.stack([packed & 15, packed >> 4], -1).reshape(6, k)
+    assert np.array_equal(int4_pack(q), packed)
+    of = np.arange(k) // group
+    step = scales.astype(np.float64)[:, of]
+    back = (q - zeros.astype(np.float64)[:, of]) * step
+    assert (np.abs(back - w) <= step * (0.5 + 15 * 2.0 ** -11 + 2.0 ** -20)).all()
+    assert not back[w == 0].any()
+
+
+def test_decode_graph_inputs():
+    g = DecodeGraph(5, 3, 11, 16, 4, 64, dim=256, n_heads=4, n_kv_heads=2, ffn=352, int4_group=64)
+    assert g.inputs["wk.q"] == ("u8", (128, 128)) and g.buffers["wk.q"] == 128 * 128
+    assert g.inputs["w2.scales"] == (ea.F16, (256, 6)) and g.inputs["w2.zeros"] == ("u8", (256, 6))
+    assert g.inputs["cache.k"] == (ea.F16, (11, 16, 2, 64))
+    assert g.buffers["page_table"] == 3 * 4 * 4 and g.buffers["offsets"] == 16
+    kinds = [n["kind"] for n in g.nodes]
+    assert kinds.count("int4_linear") == 7
+    assert kinds.index("kv_append") < kinds.index("prefix_attention")
+    dense = DecodeGraph(1, 1, 2, 16, 2, 64, dim=256, n_heads=4, ffn=352)
+    assert dense.inputs["wk"] == (ea.F16, (256, 256))
+    assert "int4_linear" not in [n["kind"] for n in dense.nodes]
