@@ -8,14 +8,21 @@
 // k of one n, one dword of the weight as it lies in memory, and the matrix unit does the
 // multiplying and adding while the vector unit has only the unpacking left.
 //
-// Unpacking: w & 0x000f000f is the pair (q0, q4) of f16 numbers q 2^-24, subnormal and exact; the
-// matrix unit takes them as they are.  The zero point is a second product with the constant
-// -z 2^-24, so that it costs the vector unit one instruction per group; the 2^24 are made up for
-// in the end.  The nibbles come out in the order 0 4 1 5 2 6 3 7, so x is put in that order too.
-// A lane loads 16 bytes, 32 consecutive k.  Groups of a multiple of 128 take them as they are
+// Unpacking: (w & 0x000f000f) | 0x64006400 is the pair (1024 + q0, 1024 + q4) in f16; minus
+// (1024 + z) it is exact.  (The bits w & 0x000f000f alone are q 2^-24, and the zero point can be a
+// second product; but products of subnormal factors were summed less exactly, f32 results were off
+// by 1e-5, and the time was the same.)  The nibbles come out in the order 0 4 1 5 2 6 3 7, so x is
+// put in that order too.
+// A lane holds 16 bytes, 32 consecutive k.  Groups of a multiple of 128 take them as they are
 // (instruction j contracts the k = 32 g + 8 j + e of the step, all of one group); smaller groups
 // have the four dwords of the four lane groups transposed (two v_permlane32_swap, two
 // v_permlane16_swap), after which instruction j holds 32 consecutive k.
+//
+// Loads: in the products' layout sixteen neighbouring lanes belong to sixteen rows, and a load
+// asks for 64 separate stretches of 16 bytes; what a load costs went by their number.  So four
+// neighbouring lanes load 64 bytes of one row, and LDS brings the values to the lanes of the
+// products (16 tokens, 11008 x 4096: 18.9 us without, 13.2 us with it).  Scales of up to four
+// steps come in one load, a step per lane group.
 //
 // Few rows of x: the rows of the 16-row tile are independent, so any row may stand in those that
 // hold no token.  With up to four (eight) rows, the four (two) lanes of one row load the
@@ -52,26 +59,19 @@ struct int4_dev_t {
     uint32_t       tokens_per_chunk;
 };
 
-// eight nibbles as q 2^-24 in the order 0 4 1 5 2 6 3 7
-__device__ inline half8_t unpack(uint32_t w)
+// eight nibbles as q - z in the order 0 4 1 5 2 6 3 7; zz = (1024 + z, 1024 + z)
+__device__ inline half8_t unpack(uint32_t w, half2_t zz)
 {
     union {
         uint32_t u[4];
+        half2_t  p[4];
         half8_t  v;
     } r;
 #pragma unroll
-    for (int i = 0; i != 4; ++i) r.u[i] = (w >> (4 * i)) & 0x000f000fu;
-    return r.v;
-}
-
-// eight times -z 2^-24
-__device__ inline half8_t minus(uint32_t z)
-{
-    union {
-        uint32_t u[4];
-        half8_t  v;
-    } r;
-    r.u[0] = r.u[1] = r.u[2] = r.u[3] = z * 0x10001u + 0x80008000u;
+    for (int i = 0; i != 4; ++i) {
+        r.u[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+        r.p[i] = r.p[i] - zz;
+    }
     return r.v;
 }
 
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
                 if (!WIDE) wt[i] = transpose_groups(wt[i]);
             }
             float4_t part[MT][NT];
-            half8_t  z[NT];
+            half2_t  z[NT];
             auto const product = [&](auto jj) {
                 constexpr int j = decltype(jj)::value;
                 // the first and the last product of a group (of what a step has of it)
@@ -358,8 +358,11 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
                 if (PARTIAL && !WIDE && st * 128 + uint32_t(j) * 32 >= k) return;
 #pragma unroll
                 for (int i = 0; i != NT; ++i) {
-                    if (first) z[i] = minus(su[u][i].zero(j / EACH));
-                    half8_t const q = unpack(wt[i][j]);
+                    if (first) {
+                        uint32_t const zero = su[u][i].zero(j / EACH) * 0x10001u + 0x64006400u;
+                        z[i] = __builtin_bit_cast(half2_t, zero);
+                    }
+                    half8_t const q = unpack(wt[i][j], z[i]);
 #pragma unroll
                     for (int t = 0; t != MT; ++t) {
                         u32x4_t f = xs[t][j / SPREAD];
@@ -367,8 +370,6 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
                         if constexpr (XL == 2) f = from_quad<j % 2 ? 0xf5 : 0xa0>(f);
                         half8_t const x = __builtin_bit_cast(half8_t, f);
                         if (first) part[t][i] = float4_t{0, 0, 0, 0};
-                        part[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, z[i], part[t][i], 0,
-                                                                           0, 0);
                         part[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q, part[t][i], 0, 0,
                                                                            0);
                         if (last) {
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
             for (int q = 0; q != WK; ++q) s += lds[q].sums[t * PARTS + p][col];
             v = v * 0x1p-11f + s;
         }
-        v = __builtin_ldexpf(v, 24 + (PARTS > 1 ? a.x_exp[token0 + t] : 0));
+        if (PARTS > 1) v = __builtin_ldexpf(v, a.x_exp[token0 + t]);
         if (n0 + col < a.n) {
             static_cast<T*>(a.y)[uint64_t(token0 + t) * a.y_stride + n0 + col] = T(v);
         }

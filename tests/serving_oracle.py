@@ -144,18 +144,14 @@ def int4_pack(q):
 
 
 def int4_64(q, scales, zeros, x, group, dtype):
-    """(y, bound): products are exact.  q x and z x are separate products: of a step of 128 k (or
-    of the part of it that is one group) 256 are summed by matrix instructions, each sum rounded
-    in units of what was added up so far; a wavefront adds its steps' sums (each multiplied by
-    its scale: one more rounding) and 8 or 16 wavefronts are joined: 256 + 1 + k / 128 + 16
-    roundings at most, relative to the magnitudes of all the products."""
+    """(y, bound): products are exact; a group's 128 (or fewer) products are summed by four
+    matrix instructions, a wavefront adds at most k / 1024 such sums and eight or sixteen are joined."""
     of = np.arange(q.shape[1]) // group
     z = 8.0 if zeros is None else zeros.astype(np.float64)[:, of]
     w = (q.astype(np.float64) - z) * scales.astype(np.float64)[:, of]
     x = x.astype(np.float64)
-    y = x @ w.T
-    mag = np.abs(x) @ ((q.astype(np.float64) + z) * np.abs(scales.astype(np.float64)[:, of])).T
-    depth = 257 + q.shape[1] / 128 + 16
+    y, mag = x @ w.T, np.abs(x) @ np.abs(w).T
+    depth = 128 + q.shape[1] / 1024 + 16
     extra = 3 if dtype == ea.F32 else 0   # three parts: joining them, and 2^-33 of x left out
     return y, (depth + extra) * U32 * mag + HALF[dtype] * np.abs(y) * 1.01 + TINY[dtype]
 
