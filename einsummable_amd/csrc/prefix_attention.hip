@@ -44,6 +44,7 @@ namespace
 {
 
 constexpr int THREADS = 256;
+constexpr int FEW = 16;
 constexpr int WAVES = THREADS / 64;
 
 struct attention_dev_t {
@@ -87,6 +88,17 @@ __device__ inline int wave_scan(int v)
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // row_bcast:15
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // row_bcast:31
     return v;
+}
+
+// The largest of 64 numbers that are not negative, in lane 63.
+__device__ inline int wave_max(int v)
+{
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true));
+    return max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true));
 }
 
 // Maximum and sum over the four lanes that share a column (lane % 16).
@@ -246,12 +258,14 @@ __device__ inline void measure(attention_dev_t const& a, int b, int e, int len, 
     per = max(1, (steps + a.grain - 1) / a.grain);
 }
 
-// Units per piece.  A multiple of four steps: one for each wavefront that takes them in turn.
+// Units per piece.  With few rows a multiple of four steps: one for each wavefront that takes them
+// in turn.
+template <int ROWS>
 __device__ inline int units_per_piece(attention_dev_t const& a, int total)
 {
     if (a.shares == 0) return 0x3fffffff;
     int const each = max(1, (total + a.shares - 1) / a.shares);
-    return a.grain % WAVES ? (each + WAVES - 1) / WAVES * WAVES : each;
+    return ROWS == FEW && a.grain % WAVES ? (each + WAVES - 1) / WAVES * WAVES : each;
 }
 
 // The piece that `item` numbers; false: there is none.  The same in all lanes.
@@ -270,7 +284,25 @@ __device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int 
             slen = a.lens[lane];
             measure<ROWS, KS>(a, sb, se, slen, tiles, per);
         }
-        each = units_per_piece(a, __builtin_amdgcn_readlane(wave_scan(tiles * per), 63));
+        each = units_per_piece<ROWS>(a, __builtin_amdgcn_readlane(wave_scan(tiles * per), 63));
+        if (ROWS != FEW) {
+            // The least size of which the batch has at most `shares` pieces, rests included, so
+            // that all run at once and there are fewer to join (prompts: 58 us where rests came
+            // second, 56 us).  More tiles than that: several rounds anyway.
+            int const count = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+            int       most = __builtin_amdgcn_readlane(wave_max(tiles > 0 ? per : 0), 63);
+            if (count <= a.shares) {
+                while (each < most) {
+                    int const mid = (each + most) / 2;
+                    int const pieces = tiles * ((per + mid - 1) / mid);
+                    if (__builtin_amdgcn_readlane(wave_scan(pieces), 63) <= a.shares) {
+                        most = mid;
+                    } else {
+                        each = mid + 1;
+                    }
+                }
+            }
+        }
         int const whole = tiles * (per / each), rest = tiles * (per % each != 0);
         int const whole_n = wave_scan(whole), rest_n = wave_scan(rest);
         wholes = __builtin_amdgcn_readlane(whole_n, 63);
@@ -305,7 +337,7 @@ __device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int 
         if (lane == 63) sh.sums[0][w] = units;
         if (tid == 0) sh.found[0] = -1;
         __syncthreads();
-        each = units_per_piece(a, sh.sums[0][0] + sh.sums[0][1] + sh.sums[0][2] + sh.sums[0][3]);
+        each = units_per_piece<ROWS>(a, sh.sums[0][0] + sh.sums[0][1] + sh.sums[0][2] + sh.sums[0][3]);
         int whole = 0, rest = 0;
         for (int s = s0; s < s1; ++s) {
             if (run > 1) read(s);
@@ -674,7 +706,6 @@ __device__ inline void raise(float top, float& m, float& ref, float& l, float4_t
 
 // ------------------------------------------------------------------------------ few rows
 
-constexpr int FEW = 16;
 
 template <typename T, int D>
 struct few_shared_t {
