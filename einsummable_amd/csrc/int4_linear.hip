@@ -513,11 +513,16 @@ void launch_columns(int4_dev_t const& a, uint64_t group, hipStream_t stream)
     // one; one token, 4096 x 11008, 2.7 tiles: 8.4 us one by one, 8.8 us in twos).
     if (tiles >= 1024) {
         launch_groups<T, PARTS, MT, 2, XL, 8>(a, group, stream);
-    } else if (MT <= 2 && tiles <= 256) {
-        launch_groups<T, PARTS, MT, 1, XL, MT <= 2 ? 16 : 8>(a, group, stream);
-    } else {
-        launch_groups<T, PARTS, MT, 1, XL, 8>(a, group, stream);
+        return;
     }
+    // (64 rows of x leave sixteen wavefronts no registers)
+    if constexpr (MT <= 2) {
+        if (tiles <= 256) {
+            launch_groups<T, PARTS, MT, 1, XL, 16>(a, group, stream);
+            return;
+        }
+    }
+    launch_groups<T, PARTS, MT, 1, XL, 8>(a, group, stream);
 }
 
 template <typename T, int PARTS>

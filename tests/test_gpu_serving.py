@@ -401,3 +401,117 @@ def test_int4_rows_do_not_touch_each_other(km, dtype):
     for i in (0, 2, 3, 5):
         assert_bits_equal(got[i], clean[i], "row %d" % i)
     assert not np.isfinite(got[1]).any() and np.isnan(got[4]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("m,k,n,group", [
+    (1, 160, 16390, 32), (2, 224, 16384, 64), (4, 160, 16417, 96), (8, 256, 16400, 128),
+    (12, 96, 16391, 64), (24, 160, 8205, 32), (64, 128, 16385, 128), (67, 160, 8200, 160)])
+def test_int4_many_columns(km, dtype, m, k, n, group):
+    got, want, bound = run_int4(km, 47, dtype, m, k, n, group, zeros=(0, 15), pad=1)
+    assert_within(got, want, bound, "int4, many columns")
+
+
+# ------------------------------------------------------------------------------ streams, sizes
+
+def test_attention_many_rows_of_many_sequences(km):
+    """Tiles of 64 and 128 rows with more sequences than lanes, and than threads."""
+    for n_seqs, heads, most in ((70, 16, 5), (300, 32, 6)):
+        r = np.random.RandomState(n_seqs)
+        new = [int(x) for x in r.randint(0, most + 1, n_seqs)]
+        lens = [n + int(x) for n, x in zip(new, r.randint(0, 90, n_seqs))]
+        run_attention(km, Paged(33, F16, heads, 1, 64, 16, new, lens))
+
+
+def test_cache_offsets_beyond_32_bits(km):
+    """Pages 3 GiB apart: entries of the last pages lie behind 2^32 elements.  The bytes of a
+    compact cache."""
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    b = Paged(34, F16, 8, 2, 128, 16, [1, 4, 1], [60, 37, 20], shared=17)
+    b.n_pages = b.k.shape[0]
+    assert b.n_pages <= 12
+    page = 16 * 2 * 128
+    far = 3 << 29
+    assert (b.n_pages - 1) * far > 1 << 32
+    near = OnDevice(b)
+    q = dev(b.r.normal(0, 1, (6, 8, 128)).astype(np.float16))
+    k = dev(b.r.normal(0, 1, (6, 2, 128)).astype(np.float16))
+    wide = torch.empty((b.n_pages - 1) * far + page, dtype=torch.float16, device="cuda")
+    pages = [wide[p * far:p * far + page].view(16, 2, 128) for p in range(b.n_pages)]
+    outs = []
+    for base, stride in ((near.k, page), (wide, far)):
+        if base is wide:
+            fresh = OnDevice(b)
+            for p in range(b.n_pages):
+                pages[p].copy_(fresh.k[p])
+        cache = ea.KvCache(F16, 8, 2, 128, b.n_pages, 16, base.data_ptr(), base.data_ptr(),
+                           (stride, 256, 128))
+        # keys and values share the buffer: a value written last is read as both
+        km.kv_append(cache, near.batch, stream_handle(), 0, 0, k.data_ptr(), k.data_ptr(), NONE)
+        need = km.prefix_attention_workspace(cache, 3, 6, 17)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        out = torch.zeros_like(q)
+        km.prefix_attention(cache, near.batch, 17, 0.09, stream_handle(), out.data_ptr(),
+                            q.data_ptr(), (ws.data_ptr(), need))
+        torch.cuda.synchronize()
+        outs.append(out.cpu().numpy())
+    assert_bits_equal(outs[1], outs[0], "attention")
+    for p in range(b.n_pages):
+        assert_bits_equal(pages[p].cpu().numpy(), near.k[p].cpu().numpy(), "page %d" % p)
+    assert outs[0].any()
+
+
+def test_calls_at_once_on_two_streams(km):
+    """Attention, append and int4 products in flight on two streams, a workspace each: the bytes
+    of one after the other."""
+    import torch
+
+    def job(seed):
+        b = Paged(seed, F16, 8, 2, 128, 16, [1, 2] * 10, [200 + 31 * i for i in range(20)],
+                  shared=128)
+        g = OnDevice(b)
+        r = b.r
+        q = dev(r.normal(0, 1, (30, 8, 128)).astype(np.float16))
+        kv = dev(r.normal(0, 1, (30, 2, 128)).astype(np.float16))
+        w = dev(r.randint(0, 256, (1024, 512)).astype(np.uint8))
+        s = dev(r.uniform(0.01, 0.02, (1024, 8)).astype(np.float32))
+        x = dev(r.normal(0, 1, (30, 1024)).astype(np.float32))
+        wt = ea.Int4Weight(F32, 1024, 1024, 128, w.data_ptr(), s.data_ptr())
+        need = (km.prefix_attention_workspace(g.cache, 20, 30, 128),
+                km.int4_linear_workspace(wt, 30))
+        ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in need]
+        out, y = torch.zeros_like(q), torch.zeros(30, 1024, device="cuda")
+
+        def go(stream):
+            for _ in range(4):
+                km.kv_append(g.cache, g.batch, stream, 0, 0, kv.data_ptr(), kv.data_ptr(), NONE)
+                km.prefix_attention(g.cache, g.batch, 128, 0.1, stream, out.data_ptr(),
+                                    q.data_ptr(), (ws[0].data_ptr(), need[0]))
+                km.int4_linear(wt, 30, stream, y.data_ptr(), x.data_ptr(),
+                               (ws[1].data_ptr(), need[1]))
+
+        def take():
+            got = out.cpu().numpy(), y.cpu().numpy(), g.k.cpu().numpy()
+            out.zero_()
+            y.zero_()
+            return got
+        go.keep = (g, q, kv, w, s, x, ws)
+        return go, take
+
+    jobs = [job(35), job(36)]
+    want = []
+    for go, take in jobs:
+        go(stream_handle())
+        torch.cuda.synchronize()
+        want.append(take())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for (go, _), s in zip(jobs, streams):
+        go(s.cuda_stream)
+    torch.cuda.synchronize()
+    for (_, take), first in zip(jobs, want):
+        for a, c in zip(take(), first):
+            assert_bits_equal(a, c, "two streams")
