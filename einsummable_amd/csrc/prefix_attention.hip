@@ -1556,6 +1556,11 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (n_seqs == 0 || n_tokens == 0) return p;
     uint64_t const kv = uint64_t(c.n_kv_heads), group = uint64_t(c.n_heads / c.n_kv_heads);
     uint64_t const rows = uint64_t(n_tokens) * group;
+    // a launch holds less than 2^32 threads; the join takes up to 64 of them for a row
+    auto const too_many = []() {
+        throw ir_error("prefix_attention: more rows (tokens times heads) than a launch holds");
+    };
+    if (rows * kv >= (1ull << 32) / 64) too_many();
     uint64_t const seqs = uint64_t(std::min(n_seqs, n_tokens));  // that have tokens, at most
     uint64_t       part_rows = 0;
     p.own_rows = tile_rows(c, rows / seqs);
@@ -1587,6 +1592,8 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     p.shares = tiles * kv >= 4 * aim ? 0 : uint32_t(std::max<uint64_t>(1, aim / kv));
     p.own_slots = uint32_t(tiles + p.shares);
     part_rows += p.own_slots * kv * p.own_rows;
+    uint64_t const units = uint64_t(p.prefix_tiles) * p.prefix_splits + p.own_slots;
+    if (units * kv >= (1ull << 32) / THREADS) too_many();
     p.part_rows = part_rows;
     p.workspace_bytes = up256(part_rows * uint64_t(padded_dim(c.head_dim)) * 4) +
                         up256(part_rows * 8) + up256(rows * 16);

@@ -178,6 +178,20 @@ def test_workspaces():
     assert sizes == sorted(sizes)
 
 
+@pytest.mark.parametrize("heads,kv,seqs,tokens", [
+    (64, 64, 1 << 20, 1 << 20),     # rows that the join's launch does not hold
+    (65536, 1, 1, 1 << 22),         # nor 32 bits
+    (32, 32, 1 << 20, 1 << 20)])    # a tile per sequence and head
+def test_batches_beyond_a_launch_are_refused(heads, kv, seqs, tokens):
+    lib, ws = ea.load_library(), ctypes.c_uint64()
+    c = cache(n_heads=heads, n_kv_heads=kv)
+    assert lib.es_km_prefix_attention_workspace(None, c._at, seqs, tokens, 0,
+                                                ctypes.addressof(ws)) == INVALID
+    assert b"than a launch holds" in lib.es_km_last_error(None)
+    assert lib.es_km_prefix_attention_workspace(None, c._at, 1 << 8, 1 << 8, 0,
+                                                ctypes.addressof(ws)) == OK
+
+
 # ------------------------------------------------------------------------------ C++ and the layer
 
 def test_cxx_members_compile(tmp_path):
