@@ -171,12 +171,16 @@ template <int MT, int NT, int XL>
 struct int4_wave_t {
     union {
         struct {
-            u32x4_t w[64];
+            u32x4_t w[128];
             u32x4_t x[XL == 4 ? 256 : 1];
         };
         float sums[MT * 4 * XL][NT * 16 + 1];
     };
 };
+
+// Where 16 bytes of row r of x lie among the row's: eight lanes that write two rows each and
+// sixteen that read sixteen rows all meet different banks.
+__device__ inline int x_swizzle(int r) { return (r & 1) * 8 + (r & 2) * 2 + r / 4; }
 
 __device__ inline void wave_sync()
 {
@@ -188,7 +192,7 @@ __device__ inline void wave_sync()
 // of a workgroup; XL: loads for a step of a row tile (1: up to four rows, 2: eight, 4: sixteen);
 // WK: wavefronts; GROUPS as above
 template <typename T, int PARTS, int MT, int NT, int XL, int WK, int GROUPS>
-__global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) void int4_kernel(int4_dev_t a)
+__global__ __launch_bounds__(64 * WK, WK == 16 || (MT * NT < 4 && GROUPS) ? 4 : 2) void int4_kernel(int4_dev_t a)
 {
     constexpr int  SPREAD = 4 / XL;  // rows of the matrix product per row of x
     constexpr bool WIDE = GROUPS == 1;
@@ -196,31 +200,38 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
     int const lane = int(threadIdx.x) & 63;
     int const w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     int const g = lane >> 4, c = lane & 15;  // as operands and results of products
-    int const q = lane >> 2, e = lane & 3;   // as loaded: four lanes read 64 bytes of a row
+    int const q = lane >> 3, e = lane & 7;   // as loaded: eight lanes read 128 bytes of a row
     uint64_t const n0 = uint64_t(blockIdx.x) * (16 * NT);
     uint32_t const token0 = blockIdx.y * a.tokens_per_chunk;
     uint32_t const rows = min(a.m - token0, a.tokens_per_chunk) * PARTS;
     uint32_t const k = uint32_t(a.k);
 
-    uint8_t const* wrow[NT];
+    uint8_t const* wrow[NT][2];  // rows q and q + 8 of the tile
     T const*       srow[NT];
     uint8_t const* zrow[NT];
 #pragma unroll
     for (int i = 0; i != NT; ++i) {
-        wrow[i] = a.w + min(n0 + uint64_t(i * 16 + q), a.n - 1) * a.w_stride + e * 16;
+#pragma unroll
+        for (int r = 0; r != 2; ++r) {
+            wrow[i][r] = a.w + min(n0 + uint64_t(i * 16 + r * 8 + q), a.n - 1) * a.w_stride;
+        }
         uint64_t const n = min(n0 + uint64_t(i * 16 + c), a.n - 1);
         srow[i] = static_cast<T const*>(a.scales) + n * a.scale_stride;
         zrow[i] = a.zeros ? a.zeros + n * a.scale_stride : int4_eights;
     }
-    _Float16 const* xrow[MT];
+    constexpr int   XR = XL == 4 ? 2 : 1;
+    _Float16 const* xrow[MT][XR];
 #pragma unroll
     for (int t = 0; t != MT; ++t) {
-        uint32_t const r = min(uint32_t(t * 16 + (XL == 4 ? q : c / SPREAD)), rows - 1);
-        xrow[t] = a.x + (uint64_t(token0) * PARTS + r) * a.x_stride;
+#pragma unroll
+        for (int i = 0; i != XR; ++i) {
+            uint32_t const r = min(uint32_t(t * 16 + (XL == 4 ? i * 8 + q : c / SPREAD)), rows - 1);
+            xrow[t][i] = a.x + (uint64_t(token0) * PARTS + r) * a.x_stride;
+        }
     }
     // k within a step of what load l brings this lane
     auto k_of = [&](int l) {
-        if (XL == 4) return uint32_t(l * 32 + e * 8);
+        if (XL == 4) return uint32_t(l / 2 * 64 + e * 8);
         int const j = l * SPREAD + c % SPREAD;
         return uint32_t(WIDE ? g * 32 + j * 8 : j * 32 + g * 8);
     };
@@ -235,7 +246,9 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
 
     uint32_t const z_mask = a.zeros ? ~0u : 0;
     int const      steps = int((k + 127) / 128), whole = int(k / 128);
-    int const      begin = steps * w / WK, end = steps * (w + 1) / WK;
+    // two steps are 128 bytes of a row
+    int const pairs = (steps + 1) / 2;
+    int const begin = pairs * w / WK * 2, end = min(steps, pairs * (w + 1) / WK * 2);
 
     // Up to U steps from st0 on, steps at stop and behind it left out.  PARTIAL: the row ends within
     // the step.
@@ -246,18 +259,23 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
         constexpr int       G = PARTIAL && GROUPS > 1 ? 0 : GROUPS;
         constexpr int       PIECES = step_scales_t<T, G>::N;
         u32x4_t             wv[U][NT];
-        u32x4_t             xv[U][MT][XL];
+        // more than a tile of x at a time leaves no registers for the x of several steps
+        constexpr int XU = MT == 1 ? U : 1;
+        u32x4_t       xv[XU][MT][XL];
         step_scales_t<T, G> sc[NT];
         // Loads without a condition, all on their way before the first is waited for: steps behind
         // the last and k behind the row stand for what is there.
 #pragma unroll
-        for (int u = 0; u != U; ++u) {
-            uint32_t const k0 = uint32_t(min(st0 + u, stop - 1)) * 128;
-            // lanes whose k the row does not have read the step's first
-            uint32_t const back = PARTIAL && k0 + uint32_t(e) * 32 >= k ? uint32_t(e) * 16 : 0;
+        for (int u = 0; u != U; u += 2) {
+            uint32_t const st = uint32_t(min(st0 + u + e / 4, stop - 1));
+            uint32_t const in = uint32_t(e % 4) * 16;
+            uint32_t const at = st * 64 + (PARTIAL && st * 128 + in * 2 >= k ? 0 : in);
 #pragma unroll
-            for (int i = 0; i != NT; ++i) {
-                wv[u][i] = *reinterpret_cast<u32x4_t const*>(wrow[i] + k0 / 2 - back);
+            for (int r = 0; r != 2; ++r) {
+#pragma unroll
+                for (int i = 0; i != NT; ++i) {
+                    wv[u + r][i] = *reinterpret_cast<u32x4_t const*>(wrow[i][r] + at);
+                }
             }
         }
         // one load for all U steps, a step per lane group
@@ -272,8 +290,7 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
 #pragma unroll
             for (int i = 0; i != NT; ++i) sc[i].load(j, srow[i], zrow[i], at, at & z_mask);
         }
-#pragma unroll
-        for (int u = 0; u != U; ++u) {
+        auto load_x = [&](int u) {
             uint32_t const k0 = uint32_t(min(st0 + u, stop - 1)) * 128;
 #pragma unroll
             for (int t = 0; t != MT; ++t) {
@@ -281,10 +298,13 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
                 for (int l = 0; l != XL; ++l) {
                     uint32_t at = k0 + k_of(l);
                     if (PARTIAL) at = at < k ? at : 0;
-                    xv[u][t][l] = *reinterpret_cast<u32x4_t const*>(xrow[t] + at);
+                    xv[u % XU][t][l] =
+                        *reinterpret_cast<u32x4_t const*>(xrow[t][l % XR] + at);
                 }
             }
-        }
+        };
+#pragma unroll
+        for (int u = 0; u != XU; ++u) load_x(u);
         __builtin_amdgcn_sched_barrier(0);
         step_scales_t<T, G> su[U][NT];
 #pragma unroll
@@ -307,13 +327,14 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
         for (int u = 0; u != U; ++u) {
             uint32_t const st = uint32_t(st0 + u);
             if (int(st) >= stop) break;
+            if (XU == 1 && u > 0) load_x(u);
             if (PARTIAL) {
 #pragma unroll
                 for (int l = 0; l != XL; ++l) {
                     bool const in = st * 128 + k_of(l) < k;
 #pragma unroll
                     for (int t = 0; t != MT; ++t) {
-                        xv[u][t][l] = in ? xv[u][t][l] : u32x4_t{0, 0, 0, 0};
+                        xv[u % XU][t][l] = in ? xv[u % XU][t][l] : u32x4_t{0, 0, 0, 0};
                     }
                 }
             }
@@ -323,29 +344,41 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
 #pragma unroll
             for (int t = 0; t != MT; ++t) {
 #pragma unroll
-                for (int l = 0; l != XL; ++l) xs[t][l] = in_nibble_order(xv[u][t][l]);
+                for (int l = 0; l != XL; ++l) xs[t][l] = in_nibble_order(xv[u % XU][t][l]);
                 if constexpr (XL == 4) {
                     wave_sync();
 #pragma unroll
                     for (int l = 0; l != 4; ++l) {
-                        mine.x[q * 16 + ((l * 4 + e) ^ (4 * (q & 3) + q / 4))] = xs[t][l];
+                        int const r = l % 2 * 8 + q;
+                        mine.x[r * 16 + ((l / 2 * 8 + e) ^ x_swizzle(r))] = xs[t][l];
                     }
                     wave_sync();
 #pragma unroll
                     for (int j = 0; j != 4; ++j) {
                         int const s = WIDE ? g * 4 + j : j * 4 + g;
-                        xs[t][j] = mine.x[c * 16 + (s ^ (4 * (c & 3) + c / 4))];
+                        xs[t][j] = mine.x[c * 16 + (s ^ x_swizzle(c))];
+                    }
+                }
+            }
+            if (u % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i != NT; ++i) {
+                    wave_sync();
+#pragma unroll
+                    for (int r = 0; r != 2; ++r) {
+                        mine.w[(r * 8 + q) * 8 + (e ^ (r * 4 + q / 2))] = wv[u + r][i];
+                    }
+                    wave_sync();
+#pragma unroll
+                    for (int r = 0; r != 2; ++r) {
+                        wv[u + r][i] = mine.w[c * 8 + ((r * 4 + g) ^ c / 2)];
                     }
                 }
             }
             u32x4_t wt[NT];
 #pragma unroll
             for (int i = 0; i != NT; ++i) {
-                wave_sync();
-                mine.w[q * 4 + (e ^ q / 4)] = wv[u][i];
-                wave_sync();
-                wt[i] = mine.w[c * 4 + (g ^ c / 4)];
-                if (!WIDE) wt[i] = transpose_groups(wt[i]);
+                wt[i] = WIDE ? wv[u][i] : transpose_groups(wv[u][i]);
             }
             float4_t part[MT][NT];
             half2_t  z[NT];
@@ -386,12 +419,12 @@ __global__ __launch_bounds__(64 * WK, WK == 16 || (MT < 4 && GROUPS) ? 4 : 2) vo
             product(std::integral_constant<int, 3>{});
         }
     };
-    constexpr int U = MT * XL * NT <= 2 ? 4 : MT * XL <= 4 ? 2 : 1;  // steps in flight
+    constexpr int U = MT * XL * NT <= 2 ? 4 : 2;  // steps in flight
     for (int st = begin; st < min(end, whole); st += U) {
         batch(st, min(end, whole), std::integral_constant<int, U>{}, std::false_type{});
     }
     if (begin < end && end > whole) {
-        batch(whole, end, std::integral_constant<int, 1>{}, std::true_type{});
+        batch(whole, end, std::integral_constant<int, 2>{}, std::true_type{});
     }
     wave_sync();
     // results: row 4 g + r, column c
