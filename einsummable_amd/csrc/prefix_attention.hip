@@ -1245,6 +1245,20 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             float4_t(&next)[NT][ST] = s[(SLOT + 1) & 1];
             wait_loads<2 * LPT*(NS - 3)>();
             __syncthreads();
+            // What is read from LDS is asked for well before its use, in an order that the
+            // scheduler may not change: K of the next tile before the addresses of later ones are
+            // worked out, V before the weights.
+            constexpr int NEXT = (SLOT + 1) % NS, NI = D / 32, PK = NI < 2 ? NI : 2, PV = 4;
+            half8_t       kf[PK][ST];
+            auto          read_k = [&](int i) {
+#pragma unroll
+                for (int t = 0; t != ST; ++t) {
+                    kf[i % PK][t] = sh.k[NEXT][16 * t + c][(4 * i + g) ^ (c & (CH - 1))];
+                }
+            };
+#pragma unroll
+            for (int i = 0; i != PK; ++i) read_k(i);
+            __builtin_amdgcn_sched_barrier(0);
             // tile + NS - 1 goes where the last one was; windows are prepared on the way
             int const j = tile + NS - 1;
             load_tile(j);
@@ -1256,44 +1270,68 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             }
             aim(j + 1);
             if (first + tile * KT > most) return;
-            scores((SLOT + 1) % NS, next);
-            half8_t p[NT][KT / 32];
-#pragma unroll
-            for (int n = 0; n != NT; ++n) {
-#pragma unroll
-                for (int t = 0; t != ST; ++t) {
-#pragma unroll
-                    for (int r = 0; r != 4; ++r) {
-                        p[n][t / 2][4 * (t & 1) + r] =
-                            T(exp2_fast(now[n][t][r] * a.scale - ref[n]));
-                    }
-                }
-            }
             // V^T: lane i of sixteen asks for four elements of key i / 4 and gets four keys of its
             // own element
             typedef short tr_t __attribute__((ext_vector_type(4)));
-#pragma unroll
-            for (int t = 0; t != DT; ++t) {
+            union {
+                tr_t    x[2];
+                half8_t h;
+            } vf[PV][KT / 32];
+            auto read_v = [&](int t) {
 #pragma unroll
                 for (int ks = 0; ks != KT / 32; ++ks) {
-                    union {
-                        tr_t    x[2];
-                        half8_t h;
-                    } vf;
 #pragma unroll
                     for (int half = 0; half != 2; ++half) {
                         int const r = 32 * ks + 16 * half + 4 * g + (c >> 2);
                         int const chunk = (2 * t + ((c & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
                         char*     at = reinterpret_cast<char*>(&sh.v[SLOT][r][chunk]) + (c & 1) * 8;
-                        vf.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        vf[t % PV][ks].x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) tr_t*)(at));
                     }
+                }
+            };
+#pragma unroll
+            for (int n = 0; n != NT; ++n) {
+#pragma unroll
+                for (int t = 0; t != ST; ++t) next[n][t] = float4_t{0, 0, 0, 0};
+            }
+            half8_t p[NT][KT / 32];
+            // scores of the next tile and, in between, the weights of this one
+#pragma unroll
+            for (int i = 0; i != NI; ++i) {
+#pragma unroll
+                for (int t = 0; t != ST; ++t) {
 #pragma unroll
                     for (int n = 0; n != NT; ++n) {
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, p[n][ks], o[n][t], 0,
-                                                                        0, 0);
+                        next[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i % PK][t], q[n][i],
+                                                                           next[n][t], 0, 0, 0);
                     }
                 }
+                if (i + PK < NI) read_k(i + PK);
+                if (i == NI - 1) {
+#pragma unroll
+                    for (int t = 0; t != PV; ++t) read_v(t);
+                }
+                constexpr int ALL = NT * ST * 4;
+#pragma unroll
+                for (int x = ALL * i / NI; x != ALL * (i + 1) / NI; ++x) {
+                    int const n = x / (ST * 4), t = x / 4 % ST, r = x % 4;
+                    p[n][t / 2][4 * (t & 1) + r] = T(exp2_fast(now[n][t][r] * a.scale - ref[n]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 0; t != DT; ++t) {
+#pragma unroll
+                for (int ks = 0; ks != KT / 32; ++ks) {
+#pragma unroll
+                    for (int n = 0; n != NT; ++n) {
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t % PV][ks].h, p[n][ks],
+                                                                        o[n][t], 0, 0, 0);
+                    }
+                }
+                if (t + PV < DT) read_v(t + PV);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int n = 0; n != NT; ++n) {
