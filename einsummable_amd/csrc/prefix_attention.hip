@@ -694,6 +694,9 @@ struct core_t<float, D> {
     }
 };
 
+// Whether a score is so much above a row's reference that the reference has to follow.
+__device__ inline bool rises(float top, float m) { return top > m + 8.0f; }
+
 // Takes the scores of a step into a row's reference m, what exponents are taken relative to
 // (`top`: the largest of this lane's).  The reference need not be the maximum: it is raised, and
 // what was summed so far scaled down, only where a score passes it by 2^8, which leaves p below
@@ -702,7 +705,7 @@ struct core_t<float, D> {
 template <int N>
 __device__ inline void raise(float top, float& m, float& ref, float& l, float4_t* o)
 {
-    if (__any(top > m + 8.0f)) {
+    if (__any(rises(top, m))) {
         float const mn = fmaxf(m, column_max(top));
         ref = mn == NEG_INF ? 0.0f : mn;
         float const fade = exp2_fast(m - ref);
@@ -1133,9 +1136,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             }
         };
         // whether there are positions in a tile that some row may not see
-        auto edge = [&](int tile) {
+        auto edge = [&](int tile, int holes) {
             int const base = first + tile * KT;
-            return sh.holes != 0 || base < lo || base + KT > hi || base + KT - 1 > least;
+            return holes != 0 || base < lo || base + KT > hi || base + KT - 1 > least;
         };
         auto mask = [&](int tile, float4_t(&s)[NT][ST]) {
             int const base = first + tile * KT;
@@ -1163,11 +1166,20 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             }
             return top * a.scale;
         };
+        // (one test for all rows: it is hardly ever true)
         auto raise_all = [&](float4_t const(&s)[NT][ST]) {
+            float top[NT];
+            bool  more = false;
+#pragma unroll
+            for (int n = 0; n != NT; ++n) {
+                top[n] = top_of(s[n]);
+                more |= rises(top[n], m[n]);
+            }
+            if (!__any(more)) return;
 #pragma unroll
             for (int n = 0; n != NT; ++n) {
                 float none = 0;
-                raise<DT + 1>(top_of(s[n]), m[n], ref[n], none, o[n]);
+                raise<DT + 1>(top[n], m[n], ref[n], none, o[n]);
             }
         };
 
@@ -1231,7 +1243,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
         clean(0);
         float4_t s[2][NT][ST];
         scores(0, s[0]);
-        if (edge(0)) mask(0, s[0]);
+        if (edge(0, sh.holes)) mask(0, s[0]);
         raise_all(s[0]);
 
         half8_t ones;
@@ -1247,7 +1259,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             __syncthreads();
             // What is read from LDS is asked for well before its use, in an order that the
             // scheduler may not change: K of the next tile before the addresses of later ones are
-            // worked out, V before the weights.
+            // worked out, V before the last weights.
             constexpr int NEXT = (SLOT + 1) % NS, NI = D / 32, PK = NI < 2 ? NI : 2, PV = 4;
             half8_t       kf[PK][ST];
             auto          read_k = [&](int i) {
@@ -1258,6 +1270,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
             };
 #pragma unroll
             for (int i = 0; i != PK; ++i) read_k(i);
+            int const holes = sh.holes;
             __builtin_amdgcn_sched_barrier(0);
             // tile + NS - 1 goes where the last one was; windows are prepared on the way
             int const j = tile + NS - 1;
@@ -1342,7 +1355,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
                 }
             }
             // (last: a branch between the scores and the values would keep them from overlapping)
-            if (edge(tile + 1)) mask(tile + 1, next);
+            if (edge(tile + 1, holes)) mask(tile + 1, next);
             raise_all(next);
         };
         for (int tile = 0; tile < tiles; tile += NS) {
