@@ -150,7 +150,8 @@ def int4_64(q, scales, zeros, x, group, dtype):
     z = 8.0 if zeros is None else zeros.astype(np.float64)[:, of]
     w = (q.astype(np.float64) - z) * scales.astype(np.float64)[:, of]
     x = x.astype(np.float64)
-    y, mag = x @ w.T, np.abs(x) @ np.abs(w).T
+    with np.errstate(invalid="ignore"):   # rows of x may hold infinities and NaN
+        y, mag = x @ w.T, np.abs(x) @ np.abs(w).T
     depth = 128 + q.shape[1] / 1024 + 16
     extra = 3 if dtype == ea.F32 else 0   # three parts: joining them, and 2^-33 of x left out
     return y, (depth + extra) * U32 * mag + HALF[dtype] * np.abs(y) * 1.01 + TINY[dtype]
