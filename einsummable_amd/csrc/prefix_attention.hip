@@ -21,7 +21,8 @@
 // workgroup take the steps of its keys in turn, straight from global memory into registers (K
 // and V are used once), and join their m, l and O at the end through LDS.  attention_many_kernel,
 // for the shared positions of a batch and for prompts: each wavefront has 16 or 32 rows of its
-// own and all of them go through the same tiles of keys, staged in LDS.
+// own and all of them go through the same tiles of keys, staged in LDS.  attention_mixed_kernel has
+// workgroups of both kinds.
 //
 // Work is cut over the keys: "prefix" workgroups take the rows of the whole batch against a cut
 // of the shared positions, the others the rows of one sequence against a cut of its own
@@ -187,10 +188,10 @@ __device__ inline void set_limit(attention_dev_t const& a, work_t const& k, int 
 // Workgroups go to the eight XCDs in turn, so with the key heads innermost every XCD gets the same
 // heads of all units: equal work however long the sequences are, and tiles that read the same keys
 // share an L2.
-__device__ inline void unit_of_block(attention_dev_t const& a, int& unit, int& kvh)
+__device__ inline void unit_of_block(attention_dev_t const& a, int block, int& unit, int& kvh)
 {
-    kvh = int(blockIdx.x) % a.h_kv;
-    unit = int(blockIdx.x) / a.h_kv;
+    kvh = block % a.h_kv;
+    unit = block / a.h_kv;
 }
 
 // A prefix workgroup: a tile of the batch's rows against a cut of the shared positions.
@@ -835,17 +836,17 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off,
     l = column_sum(l);
 }
 
+// Workgroup `block` of those that have few rows, the first prefix_units units of them the batch's.
 template <typename T, int D, bool PAD>
-__global__ __launch_bounds__(THREADS, D == 256 ? 2 : D == 128 && sizeof(T) == 4 ? 3 : 4) void attention_few_kernel(attention_dev_t a)
+__device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<T, D>& sh,
+                                         int block, int prefix_units)
 {
-    __shared__ few_shared_t<T, D> sh;
     int const tid = int(threadIdx.x), lane = tid & 63, w = tid >> 6;
     int const c = lane & 15, g = lane >> 4;
     constexpr int KS = core_t<T, D>::KS, DV = core_t<T, D>::DV;
     int           unit, kvh;
-    unit_of_block(a, unit, kvh);
-    int const prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
-    work_t    wk;
+    unit_of_block(a, block, unit, kvh);
+    work_t wk;
     if (unit < prefix_units) {
         deal_prefix<FEW>(a, unit, kvh, wk);
         prefix_limits<FEW>(a, wk, sh.limit);
@@ -1014,19 +1015,19 @@ struct many_t {
 };
 
 template <int D, int NT, bool PAD>
-__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kernel(attention_dev_t a)
+__device__ __forceinline__ void many_rows(attention_dev_t const& a,
+                                          typename many_t<D, NT>::shared_t& sh, int block,
+                                          int prefix_units)
 {
     typedef many_t<D, NT> M;
     typedef _Float16      T;
     constexpr int         ROWS = M::ROWS, KT = M::KT, CH = M::CH, DT = M::DT, NS = M::NS;
     constexpr int         LPT = M::LPT, ST = KT / 16;
-    __shared__ typename M::shared_t sh;
     int const tid = int(threadIdx.x), lane = tid & 63;
     int const w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int const c = lane & 15, g = lane >> 4;
     int       unit, kvh;
-    unit_of_block(a, unit, kvh);
-    int const  prefix_units = a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
+    unit_of_block(a, block, unit, kvh);
     bool const prefix = unit < prefix_units;
     work_t     wk;
     if (prefix) {
@@ -1424,6 +1425,46 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
     }
 }
 
+__device__ inline int prefix_units_of(attention_dev_t const& a)
+{
+    return a.parts & 1 ? a.prefix_tiles * a.prefix_splits : 0;
+}
+
+template <typename T, int D, bool PAD>
+__global__ __launch_bounds__(THREADS, D == 256 ? 2 : D == 128 && sizeof(T) == 4 ? 3 : 4) void attention_few_kernel(attention_dev_t a)
+{
+    __shared__ few_shared_t<T, D> sh;
+    few_rows<T, D, PAD>(a, sh, int(blockIdx.x), prefix_units_of(a));
+}
+
+template <int D, int NT, bool PAD>
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kernel(attention_dev_t a)
+{
+    __shared__ typename many_t<D, NT>::shared_t sh;
+    many_rows<D, NT, PAD>(a, sh, int(blockIdx.x), prefix_units_of(a));
+}
+
+// The shared positions in tiles of many rows and the own ones in tiles of few, in one launch: the
+// former are bound by instructions, the latter by memory, and two workgroups of either kind fit a
+// compute unit (64 tokens over a prefix of 8192: 22 + 31 us one after the other, 48 us together; 32
+// tokens, 32 heads of keys: 12 + 48 us, 59 us).  The former come first; in turn with the latter
+// they took 56 us.
+template <int D, int NT, bool PAD>
+__global__ __launch_bounds__(THREADS, 2) void attention_mixed_kernel(attention_dev_t a)
+{
+    __shared__ union {
+        typename many_t<D, NT>::shared_t many;
+        few_shared_t<_Float16, D>        few;
+    } sh;
+    int const units = a.prefix_tiles * a.prefix_splits, own = int(blockIdx.x) - units * a.h_kv;
+    if (own < 0) {
+        many_rows<D, NT, PAD>(a, sh.many, int(blockIdx.x), units);
+    } else {
+        few_rows<_Float16, D, PAD>(a, sh.few, own, 0);
+    }
+}
+
+
 // The references and sums of a row's cuts decide their weights, then the cuts' O are added in a
 // fixed order: TEAMS teams of sixteen lanes per row take them in turn (four teams where many cuts
 // are to be joined, one where many rows are).
@@ -1565,12 +1606,45 @@ void launch_rows(attention_dev_t a, int parts, int rows, hipStream_t stream)
     }
 }
 
+// Whether one launch takes both kinds of tiles.
+bool mixed(bool f16, int d, uint64_t prefix_splits, uint64_t prefix_rows, uint64_t own_rows)
+{
+    return f16 && d <= 128 && prefix_splits > 0 && prefix_rows > FEW && own_rows == FEW;
+}
+
+template <typename T, int D>
+bool launch_mixed(attention_dev_t const& a, hipStream_t stream)
+{
+    if constexpr (sizeof(T) == 2 && D <= 128) {
+        if (!mixed(true, a.d, uint64_t(a.prefix_splits), uint64_t(a.prefix_rows),
+                   uint64_t(a.own_rows))) {
+            return false;
+        }
+        uint32_t const grid = uint32_t((a.prefix_tiles * a.prefix_splits + a.own_slots) * a.h_kv);
+        if (a.prefix_rows == many_t<D, 2>::ROWS) {
+            if (a.d == D) {
+                attention_mixed_kernel<D, 2, false><<<grid, THREADS, 0, stream>>>(a);
+            } else {
+                attention_mixed_kernel<D, 2, true><<<grid, THREADS, 0, stream>>>(a);
+            }
+            return true;
+        }
+        if (a.d == D) {
+            attention_mixed_kernel<D, 1, false><<<grid, THREADS, 0, stream>>>(a);
+        } else {
+            attention_mixed_kernel<D, 1, true><<<grid, THREADS, 0, stream>>>(a);
+        }
+        return true;
+    }
+    return false;
+}
+
 template <typename T, int D>
 void launch_dim(attention_dev_t const& a, hipStream_t stream)
 {
     if (a.prefix_splits != 0 && a.prefix_rows == a.own_rows) {
         launch_rows<T, D>(a, 3, a.own_rows, stream);
-    } else {
+    } else if (!launch_mixed<T, D>(a, stream)) {
         if (a.prefix_splits != 0) launch_rows<T, D>(a, 1, a.prefix_rows, stream);
         launch_rows<T, D>(a, 2, a.own_rows, stream);
     }
@@ -1652,7 +1726,11 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (2 * group <= p.own_rows + 1) {
         tiles = std::min(tiles, seqs + (rows - seqs * group) / (p.own_rows - group + 1));
     }
-    uint64_t const aim = p.own_rows == FEW ? 1024 : 512;
+    // as many as run at once, two or four to a compute unit (64 tokens in one launch with the prefix:
+    // 49 us with 1024, 48 us with 512)
+    bool const     two = p.own_rows != FEW || mixed(c.dtype == ES_KM_F16, c.head_dim, p.prefix_splits,
+                                                p.prefix_rows, p.own_rows);
+    uint64_t const aim = two ? 512 : 1024;
     p.shares = tiles * kv >= 4 * aim ? 0 : uint32_t(std::max<uint64_t>(1, aim / kv));
     p.own_slots = uint32_t(tiles + p.shares);
     part_rows += p.own_slots * kv * p.own_rows;
