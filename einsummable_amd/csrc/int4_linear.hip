@@ -6,7 +6,8 @@
 // their fp32 sums through LDS in a fixed order.  The product X W^T goes through
 // v_mfma_f32_16x16x32_f16 even for one token: a lane's share of the B operand is eight consecutive
 // k of one n, one dword of the weight as it lies in memory, and the matrix unit does the
-// multiplying and adding while the vector unit has only the unpacking left.
+// multiplying and adding while the vector unit has only the unpacking left.  One token, 4096 x 11008:
+// 8.5 us, 2.8 TB/s (a read reaches 5 to 6); f32, 5 tokens, 4096 x 32000: 22 us, 3.3 TB/s.
 //
 // Unpacking: (w & 0x000f000f) | 0x64006400 is the pair (1024 + q0, 1024 + q4) in f16; minus
 // (1024 + z) it is exact.  (The bits w & 0x000f000f alone are q 2^-24, and the zero point can be a

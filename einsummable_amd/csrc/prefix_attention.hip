@@ -14,15 +14,16 @@
 // sum and scaling live in the lanes of its own column, and the four scores a lane gets of
 // sixteen keys are exactly the slice of P^T it has to supply to the second product -- for the
 // keys 4 g + r, which is then the order the lane reads the rows of V in (a sum over keys has no
-// preferred order).  Neither K nor V nor P passes through LDS.  A lane's rows of V are
-// consecutive elements of four keys; in f16 they are transposed in registers (v_perm_b32).
+// preferred order).  P passes through no memory.
 //
-// Two kernels.  attention_few_kernel, for decoding: tiles of 16 rows; the four wavefronts of a
-// workgroup take the steps of its keys in turn, straight from global memory into registers (K
-// and V are used once), and join their m, l and O at the end through LDS.  attention_many_kernel,
-// for the shared positions of a batch and for prompts: each wavefront has 16 or 32 rows of its
-// own and all of them go through the same tiles of keys, staged in LDS.  attention_mixed_kernel has
-// workgroups of both kinds.
+// Two kinds of workgroups.  attention_few_kernel, for decoding, bound by the bytes of K and V: tiles
+// of 16 rows; the four wavefronts of a workgroup take the steps of its keys in turn, straight from
+// global memory into registers (K and V are used once; in f16 a lane's four rows of V are transposed
+// there, v_perm_b32), and join their m, l and O at the end through LDS.  125 MB in 31 us, 4.0 TB/s.
+// attention_many_kernel, for the shared positions of a batch and for prompts, bound by the issue and
+// latency of its steps: each wavefront has 16 or 32 rows of its own and all of them go through the
+// same tiles of keys, staged in LDS.  30 GFLOP of prompts in 55 us, 0.55 PFLOP/s.
+// attention_mixed_kernel has workgroups of both kinds.
 //
 // Work is cut over the keys: "prefix" workgroups take the rows of the whole batch against a cut
 // of the shared positions, the others the rows of one sequence against a cut of its own
@@ -1466,8 +1467,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mixed_kernel(attention_d
 
 
 // The references and sums of a row's cuts decide their weights, then the cuts' O are added in a
-// fixed order: TEAMS teams of sixteen lanes per row take them in turn (four teams where many cuts
-// are to be joined, one where many rows are).
+// fixed order: TEAMS teams of sixteen lanes per row take them in turn: four teams where many cuts are
+// to be joined (2048 rows of 17: 7.8 us, 8.8 us with one), one where many rows are (26784 rows of two:
+// 10.1 us, 20.8 us with four).  Bound by the partial results' bytes, 17 and 41 MB.
 template <typename T, int D, int TEAMS>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t a)
 {
@@ -1705,6 +1707,8 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (shared > 0) {
         p.prefix_rows = tile_rows(c, rows);
         uint64_t const tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
+        // workgroups of few rows run four to a compute unit, and those of many are slowed by a
+        // second one (64 tokens: 22.8 us with 256, 27.4 with 384, 24.6 and 3 us more to join with 512)
         uint64_t const slots = p.prefix_rows == FEW ? 1024 : 256;
         uint64_t const want = (slots + tiles * kv - 1) / (tiles * kv);
         // no cuts below 256 positions; below 128 for a single tile of few rows, where the time is a
