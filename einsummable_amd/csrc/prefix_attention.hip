@@ -1737,7 +1737,10 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     uint64_t const aim = two ? 512 : 1024;
     p.shares = tiles * kv >= 4 * aim ? 0 : uint32_t(std::max<uint64_t>(1, aim / kv));
     p.own_slots = uint32_t(tiles + p.shares);
-    part_rows += p.own_slots * kv * p.own_rows;
+    // room for 1024 pieces of few rows either way: a batch for which both kinds of workgroups share a
+    // launch does not need less than a smaller one
+    uint64_t const room = p.own_rows == FEW ? std::max<uint64_t>(p.shares, 1024 / kv) : p.shares;
+    part_rows += (tiles + room) * kv * p.own_rows;
     uint64_t const units = uint64_t(p.prefix_tiles) * p.prefix_splits + p.own_slots;
     if (units * kv >= (1ull << 32) / THREADS) too_many();
     p.part_rows = part_rows;
