@@ -80,6 +80,18 @@ constexpr float NEG_INF = -__builtin_huge_valf();
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+__device__ inline bool finite(float x) { return x - x == 0.0f; }
+
+// y, scaled by a weight that is positive but may have underflowed: infinities stay what they are.
+__device__ inline float scaled(float y, float by) { return finite(y) ? y * by : y; }
+
+// A number that is the same in all lanes, of which the compiler is not to make two loops.
+__device__ inline int opaque(int v)
+{
+    asm volatile("" : "+s"(v));
+    return v;
+}
+
 // Inclusive sums over the 64 lanes.
 __device__ inline int wave_scan(int v)
 {
@@ -528,11 +540,6 @@ struct core_t<_Float16, D> {
             for (int i = 0; i != DV / 2; ++i) v[j].u[i] = c * DV + 2 * i < d ? v[j].u[i] : 0;
         }
     }
-    __device__ void keep_key(int j, bool keep)
-    {
-#pragma unroll
-        for (int i = 0; i != DV / 2; ++i) v[j].u[i] = keep ? v[j].u[i] : 0;
-    }
     // zeros for what is not finite; true: there was some
     __device__ bool clean_key(int j)
     {
@@ -654,17 +661,12 @@ struct core_t<float, D> {
             for (int e = 0; e != DV; ++e) v[j][e] = c * DV + e < d ? v[j][e] : 0.0f;
         }
     }
-    __device__ void keep_key(int j, bool keep)
-    {
-#pragma unroll
-        for (int i = 0; i != DV; ++i) v[j][i] = keep ? v[j][i] : 0.0f;
-    }
     __device__ bool clean_key(int j)
     {
         bool bad = false;
 #pragma unroll
         for (int e = 0; e != DV; ++e) {
-            bool const fine = v[j][e] - v[j][e] == 0.0f;
+            bool const fine = finite(v[j][e]);
             v[j][e] = fine ? v[j][e] : 0.0f;
             bad |= !fine;
         }
@@ -748,6 +750,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off,
     T const* const       kb = reinterpret_cast<T const*>(a.k) + uint64_t(kvh) * a.head_stride;
     T const* const       vb = reinterpret_cast<T const*>(a.v) + uint64_t(kvh) * a.head_stride;
     core                 x;
+    constexpr int        STEP = WAVES * KS;
     int const lo = __builtin_amdgcn_readfirstlane(wk.lo);
     int const hi = __builtin_amdgcn_readfirstlane(wk.hi);
     int const seen_by_all = __builtin_amdgcn_readfirstlane(least);
@@ -760,62 +763,80 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off,
         prow = pos - pi * a.page_size;
         page = wk.table[pi];
     };
-    constexpr int STEP = WAVES * KS;
-    int           base = (lo / KS + w) * KS;
-    float         ref = 0;
-    bool          bad = false;
-    look_up(base);
-    for (; base < hi; base += STEP) {
-        // where the keys lie, for all lanes; -1: no such page
-        int64_t const at = entry_of(a, page, prow);
-        bool const    holes = __any(at < 0);
-        __builtin_amdgcn_wave_barrier();
-        if (lane < KS) off[lane] = at;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        x.template load_k<PAD>(kb, off, c, g, a.d);
-        x.template load_v<PAD>(vb, off, c, g, a.d);
-        look_up(base + STEP);
-        // all of the step's loads go out before the first is waited for; what hides their latency
-        // is the other fifteen wavefronts of the compute unit
-        __builtin_amdgcn_sched_barrier(0);
-        x.template trim_k<PAD>(g, a.d);
-        float s[KL];
-        x.scores(s, q, lane);
-        x.template trim_v<PAD>(c, a.d);
-        bool const edge = holes || base < lo || base + KS > hi || base + KS - 1 > seen_by_all;
-        uint32_t   masked = 0;
-        if (edge) {
+    // A weight of zero -- a key that the row may not see, a position without a page, a weight that
+    // underflows -- times an infinity or NaN is no zero.  So where some row's result is not finite,
+    // the keys are gone through once more with such values made zeros, and in the end they are added
+    // to the rows that see them.
+    bool bad = false;  // some value was not finite
+    for (int careful = 0;; careful = 1) {
+        int   base = (lo / KS + w) * KS;
+        float ref = 0;
+        look_up(base);
+        for (; base < hi; base += STEP) {
+            // where the keys lie, for all lanes; -1: no such page
+            int64_t const at = entry_of(a, page, prow);
+            bool const    holes = __any(at < 0);
+            __builtin_amdgcn_wave_barrier();
+            if (lane < KS) off[lane] = at;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            x.template load_k<PAD>(kb, off, c, g, a.d);
+            x.template load_v<PAD>(vb, off, c, g, a.d);
+            look_up(base + STEP);
+            // all of the step's loads go out before the first is waited for; what hides their
+            // latency is the other fifteen wavefronts of the compute unit
+            __builtin_amdgcn_sched_barrier(0);
+            x.template trim_k<PAD>(g, a.d);
+            float s[KL];
+            x.scores(s, q, lane);
+            x.template trim_v<PAD>(c, a.d);
+            bool const edge = holes || base < lo || base + KS > hi || base + KS - 1 > seen_by_all;
+            uint32_t   masked = 0;
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j != KL; ++j) {
+                    int const key = core::key_of(j, g);
+                    masked |= off[key] < 0 || base + key < lo ||
+                                      base + key > min(hi - 1, row.limit)
+                                  ? 1u << j
+                                  : 0;
+                }
+            }
+            if (opaque(careful)) {
+#pragma unroll
+                for (int j = 0; j != KL; ++j) bad |= x.clean_key(j);
+            }
+            float top = NEG_INF;
 #pragma unroll
             for (int j = 0; j != KL; ++j) {
-                int const  key = core::key_of(j, g);
-                bool const hole = off[key] < 0;
-                // zero times an infinity or NaN is no zero: such values become zeros here and are
-                // added in the end to the rows that see them
-                x.keep_key(j, !hole);
-                bad |= x.clean_key(j);
-                masked |= hole || base + key < lo || base + key > min(hi - 1, row.limit) ? 1u << j
-                                                                                        : 0;
+                s[j] = masked >> j & 1 ? NEG_INF : s[j];
+                top = fmaxf(top, s[j]);
             }
-        }
-        float top = NEG_INF;
+            raise<DV>(top * a.scale, m, ref, l, o);
+            float sum = 0;
 #pragma unroll
-        for (int j = 0; j != KL; ++j) {
-            s[j] = masked >> j & 1 ? NEG_INF : s[j];
-            top = fmaxf(top, s[j]);
+            for (int j = 0; j != KL; ++j) {
+                s[j] = exp2_fast(s[j] * a.scale - ref);
+                sum += s[j];
+            }
+            l += sum;
+            x.values(s, o);
         }
-        raise<DV>(top * a.scale, m, ref, l, o);
-        float sum = 0;
+        if (careful) break;
+        bool again = false;
 #pragma unroll
-        for (int j = 0; j != KL; ++j) {
-            s[j] = exp2_fast(s[j] * a.scale - ref);
-            sum += s[j];
+        for (int t = 0; t != DV; ++t) {
+#pragma unroll
+            for (int r = 0; r != 4; ++r) again |= !finite(o[t][r]);
         }
-        l += sum;
-        x.values(s, o);
+        if (!__any(again && row.token >= 0)) break;
+#pragma unroll
+        for (int t = 0; t != DV; ++t) o[t] = float4_t{0, 0, 0, 0};
+        m = NEG_INF;
+        l = 0;
     }
     if (__any(bad)) {
-        for (base = (lo / KS + w) * KS; base < hi; base += STEP) {
+        for (int base = (lo / KS + w) * KS; base < hi; base += STEP) {
             for (int pos = max(base, lo); pos < min(base + KS, hi); ++pos) {
                 int const     pi = page_of(a, pos);
                 int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
@@ -826,7 +847,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off,
                     for (int r = 0; r != 4; ++r) {
                         int const   e = (4 * g + r) * DV + t;
                         float const y = float(vb[at + (!PAD || e < a.d ? e : 0)]);
-                        bool const  add = !(y - y == 0.0f) && (!PAD || e < a.d);
+                        bool const  add = !finite(y) && (!PAD || e < a.d);
                         o[t][r] += add && pos <= row.limit ? y : 0.0f;
                     }
                 }
@@ -909,7 +930,7 @@ __device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<
             int const e = (4 * g + r) * DV;
             if (D > DJ && e / DJ != h) continue;
 #pragma unroll
-            for (int t = 0; t != DV; ++t) sh.o[w][c][e - h * DJ + t] = o[t][r] * mine;
+            for (int t = 0; t != DV; ++t) sh.o[w][c][e - h * DJ + t] = scaled(o[t][r], mine);
         }
         __syncthreads();
         if (otoken >= 0) {
@@ -1008,8 +1029,8 @@ struct many_t {
         char const* kat[2][WINDOW];  // where the entries of a window's positions lie
         char const* vat[2][WINDOW];
         int         page[WINDOW];
-        int         least[WAVES];
         int         holes;  // some position has no page
+        int         again;  // some row's result is not finite
         int         bad;    // some value was not finite
         half8_t     k[NS][KT][CH], v[NS][KT][CH];
     };
@@ -1046,7 +1067,7 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
     // them would be a hot spot in the caches)
     auto inside = [&](int pos) { return min(max(pos, lo), hi - 1); };
     auto page_at = [&](int pos) { return wk.table + page_of(a, inside(pos)); };
-    int page0 = -1;
+    int  page0 = -1;
     if (lo < hi) page0 = *page_at(position(0));
 
     row_t row[NT];
@@ -1056,6 +1077,15 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
     half8_t  q[NT][D / 32];
     float4_t o[NT][DT + 1];  // [DT]: the sum of the weights, four times
     float    m[NT], ref[NT];
+    auto     start = [&]() {
+#pragma unroll
+        for (int n = 0; n != NT; ++n) {
+#pragma unroll
+            for (int t = 0; t != DT + 1; ++t) o[n][t] = float4_t{0, 0, 0, 0};
+            m[n] = NEG_INF;
+            ref[n] = 0;
+        }
+    };
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
         T const* const src = reinterpret_cast<T const*>(a.q) +
@@ -1068,11 +1098,8 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             q[n][i] = *reinterpret_cast<half8_t const*>(src + (in ? e : 0)) * T(a.q_sign);
             if (PAD && !in) q[n][i] = half8_t{};
         }
-#pragma unroll
-        for (int t = 0; t != DT + 1; ++t) o[n][t] = float4_t{0, 0, 0, 0};
-        m[n] = NEG_INF;
-        ref[n] = 0;
     }
+    start();
 
     if (lo < hi) {
         char const* const kb = a.k + uint64_t(kvh) * a.head_stride * 2;
@@ -1185,43 +1212,9 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             }
         };
 
-        if (tid == 0) sh.holes = sh.bad = 0;
-        __syncthreads();
-        put_entry(0, page0);
-        __syncthreads();
-        load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
-        // beyond the last tile too: the waits count instructions
-#pragma unroll
-        for (int i = 0; i != NS - 1; ++i) {
-            aim(i);
-            load_tile(i);
-        }
-        aim(NS - 1);
-        // while they are on their way: who sees what
-        if (prefix) prefix_limits<ROWS>(a, wk, sh.limit);
-#pragma unroll
-        for (int n = 0; n != NT; ++n) {
-            set_limit(a, wk, sh.limit, row[n]);
-            least = min(least, row[n].limit);
-            if (row[n].token >= 0) most = max(most, row[n].limit);
-        }
-#pragma unroll
-        for (int i = 1; i != 16; i <<= 1) {
-            least = min(least, __shfl_xor(least, i));
-            most = max(most, __shfl_xor(most, i));
-        }
-        least = __builtin_amdgcn_readfirstlane(least);
-        most = __builtin_amdgcn_readfirstlane(most);
-        if (lane == 0) sh.least[w] = least;
-        __syncthreads();
-        // the least limit of the workgroup's rows decides where values have to be looked at
-        int const all_see = __builtin_amdgcn_readfirstlane(
-            min(min(sh.least[0], sh.least[1]), min(sh.least[2], sh.least[3])));
-        // Zero times an infinity or NaN is no zero: where some row may not see a key of the tile,
-        // values that are not finite become zeros, and are added in the end to the rows that see
-        // them.
+        // Values that are not finite become zeros, as in attend_few.  (A second copy of the steps: in
+        // one loop for both passes the compiler needed 96 registers more.)
         auto clean = [&](int tile) {
-            if (first + tile * KT + KT - 1 <= all_see) return;
             for (int i = tid; i < KT * CH; i += THREADS) {
                 half8_t& x = sh.v[tile % NS][i / CH][i % CH];
                 half8_t  y = x;
@@ -1238,23 +1231,15 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
                     sh.bad = 1;
                 }
             }
-            __syncthreads();
         };
-        wait_loads<2 * LPT*(NS - 2)>();
-        __syncthreads();
-        clean(0);
-        float4_t s[2][NT][ST];
-        scores(0, s[0]);
-        if (edge(0, sh.holes)) mask(0, s[0]);
-        raise_all(s[0]);
-
         half8_t ones;
 #pragma unroll
         for (int e = 0; e != 8; ++e) ones[e] = T(1);
         // weights of a tile, scores of the next one, O.  SLOT, the tile's modulo NS, is known to
         // the compiler: places in LDS are then offsets of the instructions.
-        auto step = [&](int tile, auto slot_) {
-            constexpr int SLOT = decltype(slot_)::value;
+        auto step = [&](int tile, float4_t(&s)[2][NT][ST], auto slot_, auto careful_) {
+            constexpr int  SLOT = decltype(slot_)::value;
+            constexpr bool CAREFUL = decltype(careful_)::value;
             float4_t(&now)[NT][ST] = s[SLOT & 1];
             float4_t(&next)[NT][ST] = s[(SLOT + 1) & 1];
             wait_loads<2 * LPT*(NS - 3)>();
@@ -1277,7 +1262,7 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             // tile + NS - 1 goes where the last one was; windows are prepared on the way
             int const j = tile + NS - 1;
             load_tile(j);
-            clean(tile + 1);
+            if (CAREFUL) clean(tile + 1);
             int const n = j / M::TPW, at = j % M::TPW;
             if (at == M::TPW - 3) put_entry(n + 1, sh.page[tid]);
             if (at == M::TPW - 1) {
@@ -1360,15 +1345,80 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             if (edge(tile + 1, holes)) mask(tile + 1, next);
             raise_all(next);
         };
-        for (int tile = 0; tile < tiles; tile += NS) {
-            step(tile, std::integral_constant<int, 0>());
-            if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>());
-            if (tile + 2 < tiles) step(tile + 2, std::integral_constant<int, 2>());
-            if (tile + 3 < tiles) step(tile + 3, std::integral_constant<int, 3>());
+        // true: some row's result is not finite
+        auto pass = [&](auto careful_) {
+            constexpr bool CAREFUL = decltype(careful_)::value;
+            if (CAREFUL) page0 = *page_at(position(0));
+            if (tid == 0) sh.holes = sh.again = sh.bad = 0;
+            __syncthreads();
+            put_entry(0, page0);
+            __syncthreads();
+            load_to_lds_4(page_at(position(1)), lds_address(&sh.page[w * 64]));
+            // beyond the last tile too: the waits count instructions
+#pragma unroll
+            for (int i = 0; i != NS - 1; ++i) {
+                aim(i);
+                load_tile(i);
+            }
+            aim(NS - 1);
+            if (!CAREFUL) {
+                // while they are on their way: who sees what
+                if (prefix) prefix_limits<ROWS>(a, wk, sh.limit);
+#pragma unroll
+                for (int n = 0; n != NT; ++n) {
+                    set_limit(a, wk, sh.limit, row[n]);
+                    least = min(least, row[n].limit);
+                    if (row[n].token >= 0) most = max(most, row[n].limit);
+                }
+#pragma unroll
+                for (int i = 1; i != 16; i <<= 1) {
+                    least = min(least, __shfl_xor(least, i));
+                    most = max(most, __shfl_xor(most, i));
+                }
+                least = __builtin_amdgcn_readfirstlane(least);
+                most = __builtin_amdgcn_readfirstlane(most);
+            }
+            wait_loads<2 * LPT*(NS - 2)>();
+            __syncthreads();
+            if (CAREFUL) clean(0);
+            float4_t s[2][NT][ST];
+            scores(0, s[0]);
+            if (edge(0, sh.holes)) mask(0, s[0]);
+            raise_all(s[0]);
+            for (int tile = 0; tile < tiles; tile += NS) {
+                step(tile, s, std::integral_constant<int, 0>(), careful_);
+                if (tile + 1 < tiles) step(tile + 1, s, std::integral_constant<int, 1>(), careful_);
+                if (tile + 2 < tiles) step(tile + 2, s, std::integral_constant<int, 2>(), careful_);
+                if (tile + 3 < tiles) step(tile + 3, s, std::integral_constant<int, 3>(), careful_);
+            }
+            // nothing may still be on its way to LDS when it is used again, or the workgroup ends
+            wait_loads<0>();
+            if (!CAREFUL) {
+                bool again = false;
+#pragma unroll
+                for (int n = 0; n != NT; ++n) {
+#pragma unroll
+                    for (int t = 0; t != DT; ++t) {
+#pragma unroll
+                        for (int r = 0; r != 4; ++r) {
+                            again |= !finite(o[n][t][r]) && row[n].token >= 0;
+                        }
+                    }
+                }
+                if (again) sh.again = 1;
+            }
+            __syncthreads();
+            return __builtin_amdgcn_readfirstlane(sh.again) != 0;
+        };
+        bool bad = false;
+        if (pass(std::false_type())) {
+            __syncthreads();
+            start();
+            pass(std::true_type());
+            bad = sh.bad != 0;
         }
-        __syncthreads();
-        if (sh.bad) {
-            for (int pos = max(lo, (all_see - first + 1) / KT * KT + first); pos < hi; ++pos) {
+        if (bad) {
+            for (int pos = lo; pos < hi; ++pos) {
                 int const     pi = page_of(a, pos);
                 int64_t const at = entry_of(a, wk.table[pi], pos - pi * a.page_size);
                 if (at < 0) continue;
@@ -1379,7 +1429,7 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
                     for (int r = 0; r != 4; ++r) {
                         int const   e = 16 * t + 4 * g + r;
                         float const x = float(value[!PAD || e < a.d ? e : 0]);
-                        bool const  add = !(x - x == 0.0f) && (!PAD || e < a.d);
+                        bool const  add = !finite(x) && (!PAD || e < a.d);
 #pragma unroll
                         for (int n = 0; n != NT; ++n) {
                             o[n][t][r] += add && pos <= row[n].limit ? x : 0.0f;
@@ -1388,8 +1438,6 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
                 }
             }
         }
-        // nothing may still be on its way to LDS when the workgroup ends
-        wait_loads<0>();
     } else if (prefix) {
         // the page table does not reach that far
         prefix_limits<ROWS>(a, wk, sh.limit);
@@ -1527,18 +1575,20 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
                 int64_t const p = __shfl(at, which);
                 float const   fu = __shfl(f, which);
                 fi[u] = i + u * TEAMS < n ? fu : 0.0f;
-                // a cut without weight may hold anything
                 float4_t const* const src =
                     reinterpret_cast<float4_t const*>(a.part_o + p * D + lane * PER);
 #pragma unroll
                 for (int e = 0; e != PER / 4; ++e) {
-                    x[u][e] = fi[u] != 0.0f ? src[e] : float4_t{0, 0, 0, 0};
+                    x[u][e] = i + u * TEAMS < n ? src[e] : float4_t{0, 0, 0, 0};
                 }
             }
 #pragma unroll
             for (int u = 0; u != U; ++u) {
 #pragma unroll
-                for (int e = 0; e != PER / 4; ++e) y[e] += x[u][e] * fi[u];
+                for (int e = 0; e != PER / 4; ++e) {
+#pragma unroll
+                    for (int j = 0; j != 4; ++j) y[e][j] += scaled(x[u][e][j], fi[u]);
+                }
             }
         }
     }

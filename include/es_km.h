@@ -254,7 +254,8 @@ int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_b
  * that is true of the batch.  A sequence may be shorter than `shared`.
  * Positions whose page does not exist, or beyond max_pages, are left out; a token without any
  * position gets zeros.  What masked positions hold, infinities and NaN included, has no
- * influence; neither have cache entries beyond lens.
+ * influence; neither have cache entries beyond lens.  Infinities and NaN in values that a token
+ * sees reach its result whatever their weight, which is positive (and cost a second pass).
  * Batches of more tokens times heads than a launch holds (some 2^24 to 2^26) are refused.
  * q and out: n_heads heads per token, q_stride / out_stride elements from token to token, on
  * 16-byte boundaries; out may not overlap q or the cache.
