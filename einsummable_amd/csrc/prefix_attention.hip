@@ -85,6 +85,18 @@ __device__ inline bool finite(float x) { return x - x == 0.0f; }
 // y, scaled by a weight that is positive but may have underflowed: infinities stay what they are.
 __device__ inline float scaled(float y, float by) { return finite(y) ? y * by : y; }
 
+// f16 products take a weight p as two numbers, the f16 next to p and the f16 next to what that
+// leaves: 22 bits of it, where one f16 has 11 and cost results of f16 half a step of their own.  So
+// that small weights have them too, weights are taken relative to 2^-WEIGHT_LIFT of their row's
+// reference: what is lost of each is below 2^-32 of the largest.
+constexpr int WEIGHT_LIFT = 7;
+
+__device__ inline void split_weights(float2_t p, half2_t& high, half2_t& low)
+{
+    high = __builtin_convertvector(p, half2_t);
+    low = __builtin_convertvector(p - __builtin_convertvector(high, float2_t), half2_t);
+}
+
 // A number that is the same in all lanes, of which the compiler is not to make two loops.
 __device__ inline int opaque(int v)
 {
@@ -464,6 +476,7 @@ struct core_t<_Float16, D> {
     static constexpr int KL = 4;      // keys whose scores a lane holds
     static constexpr int DV = D / 16; // elements of a row of V per lane
     static constexpr int QC = D / 32;
+    static constexpr int LIFT = WEIGHT_LIFT;
 
     half8_t k[QC];
     struct vrow_t {
@@ -567,9 +580,14 @@ struct core_t<_Float16, D> {
     // o[t] += V^T P^T for the elements i * DV + t of the head, i the result's row
     __device__ void values(float const* p, float4_t* o) const
     {
-        half4_t b;
+        union {
+            half2_t pair[2];
+            half4_t h;
+        } high, low;
 #pragma unroll
-        for (int j = 0; j != KL; ++j) b[j] = _Float16(p[j]);
+        for (int j = 0; j != KL; j += 2) {
+            split_weights(float2_t{p[j], p[j + 1]}, high.pair[j / 2], low.pair[j / 2]);
+        }
 #pragma unroll
         for (int t = 0; t != DV; ++t) {
             union {
@@ -581,7 +599,8 @@ struct core_t<_Float16, D> {
             for (int i = 0; i != 2; ++i) {
                 a.u[i] = __builtin_amdgcn_perm(v[2 * i + 1].u[t / 2], v[2 * i].u[t / 2], sel);
             }
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, b, o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, high.h, o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, low.h, o[t], 0, 0, 0);
         }
     }
 };
@@ -594,6 +613,7 @@ struct core_t<float, D> {
     static constexpr int KL = 4;
     static constexpr int DV = D / 16;
     static constexpr int QC = D / 16;
+    static constexpr int LIFT = 0;
 
     float4_t k[QC];
     float    v[KL][DV];
@@ -704,15 +724,16 @@ __device__ inline bool rises(float top, float m) { return top > m + 8.0f; }
 // Takes the scores of a step into a row's reference m, what exponents are taken relative to
 // (`top`: the largest of this lane's).  The reference need not be the maximum: it is raised, and
 // what was summed so far scaled down, only where a score passes it by 2^8, which leaves p below
-// 2^8 and f16's relative precision as it is; so the lanes of a column have to agree on their
-// maximum only then.  `ref` is m, or 0 while nothing was seen.
-template <int N>
+// 2^(8 + LIFT) and f16's relative precision as it is; so the lanes of a column have to agree on their
+// maximum only then.  `ref` is m - LIFT, or anything while nothing was seen.
+template <int N, int LIFT>
 __device__ inline void raise(float top, float& m, float& ref, float& l, float4_t* o)
 {
     if (__any(rises(top, m))) {
         float const mn = fmaxf(m, column_max(top));
-        ref = mn == NEG_INF ? 0.0f : mn;
-        float const fade = exp2_fast(m - ref);
+        float const base = mn == NEG_INF ? 0.0f : mn;
+        float const fade = exp2_fast(m - base);
+        ref = base - float(LIFT);
         l *= fade;
 #pragma unroll
         for (int t = 0; t != N; ++t) o[t] *= fade;
@@ -812,7 +833,7 @@ __device__ void attend_few(attention_dev_t const& a, int64_t* off,
                 s[j] = masked >> j & 1 ? NEG_INF : s[j];
                 top = fmaxf(top, s[j]);
             }
-            raise<DV>(top * a.scale, m, ref, l, o);
+            raise<DV, core::LIFT>(top * a.scale, m, ref, l, o);
             float sum = 0;
 #pragma unroll
             for (int j = 0; j != KL; ++j) {
@@ -1012,7 +1033,6 @@ __device__ __forceinline__ uint32_t lds_address(void const* p)
 // The scores of tile i + 1 are computed in the iteration that turns those of tile i into weights:
 // the exponentials take the vector unit about as long as the matrix unit needs for the scores,
 // and in one stretch of code without dependences the two overlap.
-// The sum of a row's weights is one more row of O^T, with ones for V^T.
 template <int D, int NT>
 struct many_t {
     static constexpr int ROWS = WAVES * 16 * NT;
@@ -1075,15 +1095,15 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
     for (int n = 0; n != NT; ++n) row[n] = row_of(a, wk, kvh, (w * NT + n) * 16 + c);
 
     half8_t  q[NT][D / 32];
-    float4_t o[NT][DT + 1];  // [DT]: the sum of the weights, four times
-    float    m[NT], ref[NT];
+    float4_t o[NT][DT];
+    float    m[NT], ref[NT], l[NT];
     auto     start = [&]() {
 #pragma unroll
         for (int n = 0; n != NT; ++n) {
 #pragma unroll
-            for (int t = 0; t != DT + 1; ++t) o[n][t] = float4_t{0, 0, 0, 0};
+            for (int t = 0; t != DT; ++t) o[n][t] = float4_t{0, 0, 0, 0};
             m[n] = NEG_INF;
-            ref[n] = 0;
+            ref[n] = l[n] = 0;
         }
     };
 #pragma unroll
@@ -1207,8 +1227,7 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             if (!__any(more)) return;
 #pragma unroll
             for (int n = 0; n != NT; ++n) {
-                float none = 0;
-                raise<DT + 1>(top[n], m[n], ref[n], none, o[n]);
+                raise<DT, WEIGHT_LIFT>(top[n], m[n], ref[n], l[n], o[n]);
             }
         };
 
@@ -1232,9 +1251,6 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
                 }
             }
         };
-        half8_t ones;
-#pragma unroll
-        for (int e = 0; e != 8; ++e) ones[e] = T(1);
         // weights of a tile, scores of the next one, O.  SLOT, the tile's modulo NS, is known to
         // the compiler: places in LDS are then offsets of the instructions.
         auto step = [&](int tile, float4_t(&s)[2][NT][ST], auto slot_, auto careful_) {
@@ -1295,7 +1311,10 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
 #pragma unroll
                 for (int t = 0; t != ST; ++t) next[n][t] = float4_t{0, 0, 0, 0};
             }
-            half8_t p[NT][KT / 32];
+            union {
+                half2_t pair[4];
+                half8_t h;
+            } high[NT][KT / 32], low[NT][KT / 32];
             // scores of the next tile and, in between, the weights of this one
 #pragma unroll
             for (int i = 0; i != NI; ++i) {
@@ -1312,11 +1331,16 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
 #pragma unroll
                     for (int t = 0; t != PV; ++t) read_v(t);
                 }
-                constexpr int ALL = NT * ST * 4;
+                constexpr int ALL = NT * ST * 2;
 #pragma unroll
                 for (int x = ALL * i / NI; x != ALL * (i + 1) / NI; ++x) {
-                    int const n = x / (ST * 4), t = x / 4 % ST, r = x % 4;
-                    p[n][t / 2][4 * (t & 1) + r] = T(exp2_fast(now[n][t][r] * a.scale - ref[n]));
+                    int const n = x / (ST * 2), t = x / 2 % ST, r = x % 2;
+                    float2_t  p;
+                    p.x = exp2_fast(now[n][t][2 * r] * a.scale - ref[n]);
+                    p.y = exp2_fast(now[n][t][2 * r + 1] * a.scale - ref[n]);
+                    l[n] += p.x + p.y;
+                    split_weights(p, high[n][t / 2].pair[2 * (t & 1) + r],
+                                  low[n][t / 2].pair[2 * (t & 1) + r]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -1326,20 +1350,17 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
                 for (int ks = 0; ks != KT / 32; ++ks) {
 #pragma unroll
                     for (int n = 0; n != NT; ++n) {
-                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t % PV][ks].h, p[n][ks],
-                                                                        o[n][t], 0, 0, 0);
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            vf[t % PV][ks].h, high[n][ks].h, o[n][t], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int n = 0; n != NT; ++n) {
+                        o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            vf[t % PV][ks].h, low[n][ks].h, o[n][t], 0, 0, 0);
                     }
                 }
                 if (t + PV < DT) read_v(t + PV);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int n = 0; n != NT; ++n) {
-#pragma unroll
-                for (int ks = 0; ks != KT / 32; ++ks) {
-                    o[n][DT] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[n][ks], o[n][DT], 0, 0, 0);
-                }
             }
             // (last: a branch between the scores and the values would keep them from overlapping)
             if (edge(tile + 1, holes)) mask(tile + 1, next);
@@ -1446,12 +1467,14 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
     }
 #pragma unroll
     for (int n = 0; n != NT; ++n) {
+        // the four lanes of a column hold sums over different keys
+        l[n] = column_sum(l[n]);
         if (row[n].token < 0) continue;
         // O^T: elements 16 t + 4 g + r of this lane's row
         if (wk.direct) {
             T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(row[n].token) * a.out_stride +
                            uint64_t(row[n].head) * uint64_t(a.d);
-            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / o[n][DT][0];
+            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / l[n];
 #pragma unroll
             for (int t = 0; t != DT; ++t) {
                 int const e = 16 * t + 4 * g;
@@ -1468,7 +1491,7 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
             }
             if (g == 0) {
                 a.part_ml[at * 2] = m[n];
-                a.part_ml[at * 2 + 1] = o[n][DT][0];
+                a.part_ml[at * 2 + 1] = l[n];
             }
         }
     }
