@@ -718,6 +718,26 @@ struct core_t<float, D> {
     }
 };
 
+// The sum of a row's weights in a part, with the reference m (l: their sum, zero also where none was
+// added).  A softmax over scores that are all -inf is NaN, over no score the caller wants zeros: where
+// m is -inf and l zero, -1 says that the row saw a key all the same.  (NaN scores leave m alone and
+// make l NaN.)
+__device__ inline float sum_of(attention_dev_t const& a, work_t const& k, int limit, float m, float l)
+{
+    int const last = min(k.hi - 1, limit);
+    if (m != NEG_INF || l != 0.0f || last < k.lo) return l;
+    for (int p = page_of(a, k.lo); p <= page_of(a, last); ++p) {
+        if (entry_of(a, k.table[p], 0) >= 0) return -1.0f;
+    }
+    return l;
+}
+
+// What an element of O is multiplied with: 1 / sum, zero for a row that saw nothing.
+__device__ inline float weight_of(float sum)
+{
+    return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : __builtin_nanf("");
+}
+
 // Whether a score is so much above a row's reference that the reference has to follow.
 __device__ inline bool rises(float top, float m) { return top > m + 8.0f; }
 
@@ -935,6 +955,7 @@ __device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<
     // the row that this thread stores, from the lane that knows it
     int const   otoken = __shfl(row.token, orow);
     int const   ohead = __shfl(row.head, orow);
+    int const   olimit = __shfl(row.limit, orow);
     float const otop = __shfl(top, orow);
     float       sum = 0;
 #pragma unroll
@@ -942,6 +963,7 @@ __device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<
         float const mi = sh.m[i][orow];
         sum += sh.l[i][orow] * exp2_fast(mi - (otop == NEG_INF ? 0.0f : otop));
     }
+    sum = sum_of(a, wk, olimit, otop, sum);
 #pragma unroll
     for (int h = 0; h != D / DJ; ++h) {
         if (h) __syncthreads();
@@ -965,12 +987,12 @@ __device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<
             if (wk.direct) {
                 T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(otoken) * a.out_stride +
                                uint64_t(ohead) * uint64_t(a.d) + h * DJ + oe;
-                float const inv = otop == NEG_INF ? 0.0f : 1.0f / sum;
+                float const inv = weight_of(sum);
                 // PER divides 8, and 8 divides d: all of them or none
                 typedef T vec_t __attribute__((ext_vector_type(PER)));
                 vec_t     z;
 #pragma unroll
-                for (int e = 0; e != PER; ++e) z[e] = T(otop == NEG_INF ? 0.0f : y[e] * inv);
+                for (int e = 0; e != PER; ++e) z[e] = T(y[e] * inv);
                 if (h * DJ + oe < a.d) *reinterpret_cast<vec_t*>(dst) = z;
             } else {
                 float* const dst = a.part_o + (wk.part + orow) * D + h * DJ + oe;
@@ -1470,17 +1492,18 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
         // the four lanes of a column hold sums over different keys
         l[n] = column_sum(l[n]);
         if (row[n].token < 0) continue;
+        l[n] = sum_of(a, wk, row[n].limit, m[n], l[n]);
         // O^T: elements 16 t + 4 g + r of this lane's row
         if (wk.direct) {
             T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(row[n].token) * a.out_stride +
                            uint64_t(row[n].head) * uint64_t(a.d);
-            float const inv = m[n] == NEG_INF ? 0.0f : 1.0f / l[n];
+            float const inv = weight_of(l[n]);
 #pragma unroll
             for (int t = 0; t != DT; ++t) {
                 int const e = 16 * t + 4 * g;
                 half4_t   y;
 #pragma unroll
-                for (int r = 0; r != 4; ++r) y[r] = T(m[n] == NEG_INF ? 0.0f : o[n][t][r] * inv);
+                for (int r = 0; r != 4; ++r) y[r] = T(o[n][t][r] * inv);
                 if (e < a.d) *reinterpret_cast<half4_t*>(dst + e) = y;
             }
         } else {
@@ -1580,13 +1603,14 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
     for (int e = 0; e != PER / 4; ++e) y[e] = float4_t{0, 0, 0, 0};
     int const group0 = int(threadIdx.x) & 63 & ~(LANES - 1);
     for (int i0 = 0; i0 < parts; i0 += LANES) {
-        // lane i: the place and the weight of cut i0 + i; none without keys for this row
+        // lane i: the place and the weight of cut i0 + i; none without keys for this row, or with
+        // scores of -inf only beside a cut of others
         bool const    in = i0 + lane < parts;
         int64_t const at = in ? place(i0 + lane) : 0;
         float const   mi = in ? a.part_ml[at * 2] : NEG_INF;
         float const   li = in ? a.part_ml[at * 2 + 1] : 0.0f;
         float const   f = mi == NEG_INF ? 0.0f : exp2_fast(mi - top);
-        sum += mi == NEG_INF ? 0.0f : li * f;
+        sum += mi != NEG_INF ? li * f : li < 0.0f && top != NEG_INF ? 0.0f : li;
         constexpr int U = 4;  // cuts in flight
         int const     n = min(parts - i0, LANES);
         for (int i = team; i < n; i += U * TEAMS) {
@@ -1628,7 +1652,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
     if (team != 0) return;
     T* const    dst = reinterpret_cast<T*>(a.out) + uint64_t(token) * a.out_stride +
                    uint64_t(head) * uint64_t(a.d) + lane * PER;
-    float const inv = top == NEG_INF ? 0.0f : 1.0f / sum;
+    float const inv = weight_of(sum);
     // in vectors of at most 16 bytes; d is a multiple of 8
     constexpr int V = PER < 16 / int(sizeof(T)) ? PER : 16 / int(sizeof(T));
     typedef T     vec_t __attribute__((ext_vector_type(V)));
@@ -1637,7 +1661,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t
         vec_t z;
 #pragma unroll
         for (int i = 0; i != V; ++i) {
-            z[i] = T(top == NEG_INF ? 0.0f : y[(e + i) / 4][(e + i) % 4] * inv);
+            z[i] = T(y[(e + i) / 4][(e + i) % 4] * inv);
         }
         if (lane * PER + e < a.d) *reinterpret_cast<vec_t*>(dst + e) = z;
     }

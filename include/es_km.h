@@ -253,7 +253,8 @@ int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_b
  * sequences together; 0 when nothing is shared.  The result is the same for every `shared`
  * that is true of the batch.  A sequence may be shorter than `shared`.
  * Positions whose page does not exist, or beyond max_pages, are left out; a token without any
- * position gets zeros.  What masked positions hold, infinities and NaN included, has no
+ * position gets zeros; one that sees a NaN score, or no other score than -inf, gets NaN, as the
+ * formula does.  What masked positions hold, infinities and NaN included, has no
  * influence; neither have cache entries beyond lens.  Infinities and NaN in values that a token
  * sees reach its result whatever their weight, which is positive (and cost a second pass).
  * Scores, weights, sums and results are fp32; in f16 the matrix unit gets each weight as two f16

@@ -136,3 +136,72 @@ def test_rows_that_see_no_infinity_keep_every_bit(km):
         keep = [i for i in range(b.d) if i != 3]
         assert_bits_equal(got[last][:, keep], clean[last][:, keep], "other elements")
         assert np.isposinf(got[last, :, 3]).all()
+
+
+# one own position each, behind the prefix: parts that hold a single key
+ALONE = [(4, 2, 128, 8, [1] * 40, [71] * 40, 70), (4, 2, 64, 8, [1] * 3, [71] * 3, 70),
+         (8, 1, 128, 16, [5] * 8, [75] * 8, 70)]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", SHAPES + ALONE, ids=lambda s: "h%d-%d-d%d-t%d-s%d" %
+                         (s[0], s[1], s[2], sum(s[4]), s[6]))
+def test_nan_scores_reach_the_result(km, dtype, shape):
+    """NaN in a query, and in keys that a row sees; all other rows keep every bit."""
+    shared = shape[-1]
+    for part in (shared, 0):
+        b = Paged(73, dtype, *shape)
+        q, scale = queries(b), b.d ** -0.5
+        clean = attend(km, b, q, scale, part)
+        bad = q.copy()
+        bad[b.used // 2, 1, 5] = np.nan
+        got = attend(km, b, bad, scale, part)
+        assert np.isnan(got[b.used // 2, 1]).all()
+        got[b.used // 2, 1] = clean[b.used // 2, 1]
+        assert_bits_equal(got, clean, "NaN in a query")
+        # the newest key of each sequence in turn; all keys of the first one's; a shared one
+        for s in (0, b.n_seqs - 1):
+            b = Paged(73, dtype, *shape)
+            put(b, b.k, b.lens[s] - 1, 5, np.nan, [s])
+            last = int(b.offsets[s + 1]) - 1
+            got = attend(km, b, q, scale, part)
+            assert np.isnan(got[last]).all()
+            got[last] = clean[last]
+            assert_bits_equal(got, clean, "NaN in the newest key")
+        for pos in range(shared, b.lens[0]):
+            put(b, b.k, pos, 0, np.nan, [0])
+        got = attend(km, b, q, scale, part)
+        b = Paged(73, dtype, *shape)
+        put(b, b.k, shared - 1, 5, np.nan)
+        assert np.isnan(got[b.new[0] - 1]).all()
+        assert np.isnan(attend(km, b, q, scale, part)).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("new,lens,shared", [
+    ([1, 1, 2], [40, 1, 35], 0), ([1] * 40, [70] * 40, 33), ([70, 30], [70, 40], 0),
+    ([9] * 8, [50] * 8, 33)])
+def test_scores_of_minus_infinity(km, dtype, new, lens, shared):
+    """Weight zero, as if there were no such key; a row that sees no other has no softmax: NaN."""
+    b = Paged(74, dtype, 4, 1, 64, 1, new, lens, shared)
+    q = queries(b)
+    q[..., 0] = 1
+    b.k[..., 0] = 0
+    gone = Paged(74, dtype, 4, 1, 64, 1, new, lens, shared)
+    gone.k[..., 0] = 0
+    r = np.random.RandomState(0)
+    for s in range(b.n_seqs):
+        at = np.arange(shared, lens[s])
+        at = at if s % 3 == 0 else r.permutation(at)[:at.size // 2]
+        b.k[b.table[s, at], 0, :, 0] = -np.inf
+        gone.table[s, at] = -1
+    first = attend(km, b, q, 0.1)
+    want, bound = attention64(gone, q, 0.1)
+    for s in range(b.n_seqs):
+        rows = slice(int(b.offsets[s]), int(b.offsets[s + 1]))
+        sees = (gone.table[s, :lens[s]] >= 0).cumsum()[lens[s] - new[s]:lens[s]] > 0
+        assert np.isnan(first[rows][~sees]).all()
+        assert_within(first[rows][sees], want[rows][sees], bound[rows][sees], "keys of weight zero")
+    # no position at all: zeros
+    b.table[:] = -1
+    assert not attend(km, b, q, 0.1).any()
