@@ -219,6 +219,32 @@ __device__ inline void unit_of_block(attention_dev_t const& a, int block, int& u
     unit = block / a.h_kv;
 }
 
+// The sequence through whose row of the page table the shared positions are read: one that has
+// tokens and maps them all, the first if it does; if none does, the longest, beyond which no row sees
+// any.  (An idle sequence's row holds anything, and that of one that ends inside the prefix too from
+// there on.)  All lanes take part.
+__device__ inline int prefix_sequence(attention_dev_t const& a)
+{
+    int const need = min(a.shared, a.max_pages * a.page_size);
+    auto      length = [&](int s) {
+        bool const any = min(a.offsets[s + 1], a.n_tokens) > max(a.offsets[s], 0);
+        return any ? a.lens[s] : -1;
+    };
+    if (length(0) >= need) return 0;
+    int const lane = int(threadIdx.x) & 63;
+    int       best = -1, at = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        int const      len = s0 + lane < a.n_seqs ? length(s0 + lane) : -1;
+        uint64_t const all = __ballot(len >= need);
+        if (all) return s0 + __ffsll((unsigned long long)all) - 1;
+        at = len > best ? s0 + lane : at;
+        best = max(best, len);
+    }
+    int const longest = __builtin_amdgcn_readlane(wave_max(max(best, 0)), 63);
+    uint64_t const which = __ballot(best == longest);
+    return which ? __builtin_amdgcn_readlane(at, __ffsll((unsigned long long)which) - 1) : 0;
+}
+
 // A prefix workgroup: a tile of the batch's rows against a cut of the shared positions.
 template <int ROWS>
 __device__ inline void deal_prefix(attention_dev_t const& a, int unit, int kvh, work_t& k)
@@ -228,7 +254,7 @@ __device__ inline void deal_prefix(attention_dev_t const& a, int unit, int kvh, 
     k.part = (int64_t(unit) * a.h_kv + kvh) * ROWS;
     k.lo = split * a.prefix_chunk;
     k.hi = min(min(k.lo + a.prefix_chunk, a.shared), a.max_pages * a.page_size);
-    k.table = a.table;
+    k.table = a.table + uint64_t(prefix_sequence(a)) * a.table_stride;
     k.direct = false;
     k.whole = true;
     k.r0 = tile * ROWS;

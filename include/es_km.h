@@ -249,9 +249,10 @@ int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_b
  *   out[i, h] = sum_j p_j V[j, h'],  p = softmax_j(scale * q[i, h] . K[j, h'])
  * over the positions j of token i's sequence up to its own (h' the key head of h).  The first
  * `shared` positions hold the same keys and values for every sequence of the batch (a common
- * prefix): they are read through the page table's first row, once for the rows of many
- * sequences together; 0 when nothing is shared.  The result is the same for every `shared`
- * that is true of the batch.  A sequence may be shorter than `shared`.
+ * prefix): they are read through the page table's row of one sequence that has tokens and is
+ * that long (of the longest, where none is), once for the rows of many sequences together; 0 when
+ * nothing is shared.  The result is the same for every `shared` that is true of the batch.  A
+ * sequence may be shorter than `shared`.
  * Positions whose page does not exist, or beyond max_pages, are left out; a token without any
  * position gets zeros; one that sees a NaN score, or no other score than -inf, gets NaN, as the
  * formula does.  What masked positions hold, infinities and NaN included, has no
