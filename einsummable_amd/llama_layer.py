@@ -306,42 +306,48 @@ class DeviceRunner:
             if name not in self.mem:
                 self.mem[name] = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
             assert self.mem[name].numel() == nbytes, name
-        need = 0
+        # by node, here and not in the graph, which other runners may have too
+        self.need = []
         for n in graph.nodes:
+            ws = 0
             if n["kind"] == "einsummable":
                 ws = km.build(n["e"])
                 assert ws is not None, "no kernel for node " + n["label"]
-            elif n["kind"] in ("kv_append", "prefix_attention", "int4_linear"):
-                ws = self._serving(n)
-            else:
-                continue
-            n["ws"] = ws
-            need = max(need, ws)
+            elif n["kind"] == "int4_linear":
+                ws = km.int4_linear_workspace(self._weight(n), n["shape"][0])
+            elif n["kind"] == "prefix_attention":
+                ws = km.prefix_attention_workspace(self._cache(n), graph.n_seqs, graph.seq,
+                                                   graph.shared)
+            self.need.append(ws)
         # one scratch buffer serves every node: they run one after the other on one stream
-        self.workspace = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        self.workspace = torch.empty(max(self.need + [1]), dtype=torch.uint8, device="cuda")
 
-    def _serving(self, n):
-        """Descriptors of a serving node and its call; returns the workspace it needs."""
+    def _at(self, *names):
+        return [self.mem[name].data_ptr() for name in names]
+
+    def _weight(self, n):
+        _, n_out, n_in = n["shape"]
+        return Int4Weight(F16, n_out, n_in, n["group"], *self._at(*n["w"]))
+
+    def _cache(self, n):
+        g = self.g
+        return KvCache(F16, g.n_heads, g.n_kv, g.hd, g.n_pages, g.page_size, *self._at(*n["cache"]))
+
+    def _batch(self, n):
+        g = self.g
+        return KvBatch(g.n_seqs, g.seq, *self._at(*n["batch"]), g.max_pages)
+
+    def _serve(self, n, stream, ws):
+        """A serving node on the buffers of the moment."""
         km, g = self.km, self.g
-        at = {name: m.data_ptr() for name, m in self.mem.items()}
         if n["kind"] == "int4_linear":
-            m, n_out, n_in = n["shape"]
-            q, scales, zeros = n["w"]
-            w = Int4Weight(F16, n_out, n_in, n["group"], at[q], at[scales], at[zeros])
-            n["call"] = lambda stream, ws: km.int4_linear(w, m, stream, at[n["out"]], at[n["inn"]],
-                                                          ws)
-            return km.int4_linear_workspace(w, m)
-        cache = KvCache(F16, g.n_heads, g.n_kv, g.hd, g.n_pages, g.page_size,
-                        *[at[c] for c in n["cache"]])
-        batch = KvBatch(g.n_seqs, g.seq, *[at[b] for b in n["batch"]], g.max_pages)
-        if n["kind"] == "kv_append":
-            n["call"] = lambda stream, ws: km.kv_append(cache, batch, stream, at[n["out"]],
-                                                        *[at[b] for b in n["inns"]], ROPE_PAIRS,
-                                                        at[n["freqs"]], g.n_pos)
-            return 0
-        n["call"] = lambda stream, ws: km.prefix_attention(cache, batch, g.shared, g.scale, stream,
-                                                           at[n["out"]], at[n["inn"]], ws)
-        return km.prefix_attention_workspace(cache, g.n_seqs, g.seq, g.shared)
+            km.int4_linear(self._weight(n), n["shape"][0], stream, *self._at(n["out"], n["inn"]), ws)
+        elif n["kind"] == "kv_append":
+            km.kv_append(self._cache(n), self._batch(n), stream, *self._at(n["out"], *n["inns"]),
+                         ROPE_PAIRS, *self._at(n["freqs"]), g.n_pos)
+        else:
+            km.prefix_attention(self._cache(n), self._batch(n), g.shared, g.scale, stream,
+                                *self._at(n["out"], n["inn"]), ws)
 
     def set_input(self, name, array):
         import numpy as np
@@ -359,16 +365,17 @@ class DeviceRunner:
         km = self.km
         stream = stream if stream is not None else self.torch.cuda.current_stream().cuda_stream
         for i, n in enumerate(self.g.nodes):
-            def launch(n=n):
+            ws = (self.workspace.data_ptr(), self.need[i]) if self.need[i] else None
+
+            def launch(n=n, ws=ws):
                 if n["kind"] == "einsummable":
                     km(n["e"], stream, self.mem[n["out"]].data_ptr(),
-                       [self.mem[b].data_ptr() for b in n["inns"]],
-                       (self.workspace.data_ptr(), n["ws"]) if n["ws"] else None)
+                       [self.mem[b].data_ptr() for b in n["inns"]], ws)
                 elif n["kind"] == "touch":
                     km.touch(n["t"], stream, self.mem[n["out"]].data_ptr(),
                              self.mem[n["inn"]].data_ptr())
-                elif "call" in n:
-                    n["call"](stream, (self.workspace.data_ptr(), n["ws"]) if n["ws"] else None)
+                elif n["kind"] in ("kv_append", "prefix_attention", "int4_linear"):
+                    self._serve(n, stream, ws)
                 else:
                     assert n["dtype"] == F16
                     lo = struct.unpack("<H", struct.pack("<e", n["lower"]))[0]
