@@ -72,7 +72,7 @@ struct attention_dev_t {
     int         direct;     // there are no shared positions to join with
     float*      part_o;     // [row of a slot][D]: the prefix's slots, then the own ones
     float*      part_ml;    // [row of a slot][2]
-    int4*       part_meta;  // [token * group + head of the group], see piece()
+    int4*       part_meta;  // [token * group + head of the group], see piece(); null: no join
     int64_t     own_base;   // rows before the own positions' slots
 };
 
@@ -461,7 +461,7 @@ __device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int 
     k.direct = parts == 1 && a.direct;
     k.table = a.table + uint64_t(q.s) * a.table_stride;
     k.r0 = tile * ROWS;
-    if (at == 0 && kvh == 0) {
+    if (at == 0 && kvh == 0 && a.part_meta) {
         // where the rows' partial results are: from x on y of them, then z (or none); w the row
         for (int i = tid; i < ROWS; i += THREADS) {
             int const r = k.r0 + i, t = k.b + r / a.group;
@@ -1863,12 +1863,15 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     // room for 1024 pieces of few rows either way: a batch for which both kinds of workgroups share a
     // launch does not need less than a smaller one
     uint64_t const room = p.own_rows == FEW ? std::max<uint64_t>(p.shares, 1024 / kv) : p.shares;
-    part_rows += (tiles + room) * kv * p.own_rows;
+    // nothing is cut: each tile's result goes straight to the output
+    bool const joined = p.prefix_splits != 0 || p.shares != 0;
+    if (joined) part_rows += (tiles + room) * kv * p.own_rows;
     uint64_t const units = uint64_t(p.prefix_tiles) * p.prefix_splits + p.own_slots;
     if (units * kv >= (1ull << 32) / THREADS) too_many();
     p.part_rows = part_rows;
-    p.workspace_bytes = up256(part_rows * uint64_t(padded_dim(c.head_dim)) * 4) +
-                        up256(part_rows * 8) + up256(rows * 16);
+    p.workspace_bytes = joined ? up256(part_rows * uint64_t(padded_dim(c.head_dim)) * 4) +
+                                     up256(part_rows * 8) + up256(rows * 16)
+                               : 0;
     return p;
 }
 
@@ -1921,11 +1924,15 @@ void launch_attention(attention_args_t const& g, attention_plan_t const& p, void
     a.own_base = int64_t(p.own_base);
     a.direct = p.prefix_splits == 0;
     a.parts = 0;
-    char* const    ws = static_cast<char*>(workspace);
-    uint64_t const o_bytes = up256(p.part_rows * uint64_t(padded_dim(a.d)) * 4);
-    a.part_o = reinterpret_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float*>(ws + o_bytes);
-    a.part_meta = reinterpret_cast<int4*>(ws + o_bytes + up256(p.part_rows * 8));
+    a.part_o = a.part_ml = nullptr;
+    a.part_meta = nullptr;
+    if (p.workspace_bytes != 0) {
+        char* const    ws = static_cast<char*>(workspace);
+        uint64_t const o_bytes = up256(p.part_rows * uint64_t(padded_dim(a.d)) * 4);
+        a.part_o = reinterpret_cast<float*>(ws);
+        a.part_ml = reinterpret_cast<float*>(ws + o_bytes);
+        a.part_meta = reinterpret_cast<int4*>(ws + o_bytes + up256(p.part_rows * 8));
+    }
     if (g.cache.dtype == ES_KM_F16) {
         launch_type<_Float16>(a, stream);
     } else {

@@ -265,8 +265,9 @@ int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_b
  * 16-byte boundaries; out may not overlap q or the cache.
  * workspace: es_km_prefix_attention_workspace bytes on a 256-byte boundary, used from the
  * call until its work is done (calls that overlap in time need one each), contents irrelevant
- * before and after.  The need follows from the cuts: a batch of fewer tokens may need somewhat
- * more than a larger one, so a loop asks for each of its batch sizes. */
+ * before and after.  The need follows from the cuts: a batch of fewer tokens may need more than a
+ * larger one, and one of so many that nothing is cut needs 0 (NULL is fine then), so a loop asks for
+ * each of its batch sizes. */
 int es_km_prefix_attention_workspace(es_km_t* km, const es_km_kv_cache_t* cache, int n_seqs,
                                      int n_tokens, uint64_t shared, uint64_t* workspace_bytes);
 int es_km_prefix_attention(es_km_t* km, const es_km_kv_cache_t* cache,
