@@ -747,13 +747,19 @@ struct core_t<float, D> {
 // The sum of a row's weights in a part, with the reference m (l: their sum, zero also where none was
 // added).  A softmax over scores that are all -inf is NaN, over no score the caller wants zeros: where
 // m is -inf and l zero, -1 says that the row saw a key all the same.  (NaN scores leave m alone and
-// make l NaN.)
+// make l NaN.)  All lanes take part: they look for the part's first position with a page together.
 __device__ inline float sum_of(attention_dev_t const& a, work_t const& k, int limit, float m, float l)
 {
-    int const last = min(k.hi - 1, limit);
-    if (m != NEG_INF || l != 0.0f || last < k.lo) return l;
-    for (int p = page_of(a, k.lo); p <= page_of(a, last); ++p) {
-        if (entry_of(a, k.table[p], 0) >= 0) return -1.0f;
+    bool const none = m == NEG_INF && l == 0.0f && limit >= k.lo;
+    if (!__any(none)) return l;
+    int const lane = int(threadIdx.x) & 63;
+    for (int base = k.lo; base < k.hi; base += 64) {
+        int const      pos = min(base + lane, k.hi - 1);
+        uint64_t const there = __ballot(entry_of(a, k.table[page_of(a, pos)], 0) >= 0);
+        if (there) {
+            int const first = min(base + __ffsll((unsigned long long)there) - 1, k.hi - 1);
+            return none && limit >= first ? -1.0f : l;
+        }
     }
     return l;
 }
@@ -989,7 +995,7 @@ __device__ __forceinline__ void few_rows(attention_dev_t const& a, few_shared_t<
         float const mi = sh.m[i][orow];
         sum += sh.l[i][orow] * exp2_fast(mi - (otop == NEG_INF ? 0.0f : otop));
     }
-    sum = sum_of(a, wk, olimit, otop, sum);
+    sum = sum_of(a, wk, otoken < 0 ? -1 : olimit, otop, sum);
 #pragma unroll
     for (int h = 0; h != D / DJ; ++h) {
         if (h) __syncthreads();
@@ -1517,8 +1523,8 @@ __device__ __forceinline__ void many_rows(attention_dev_t const& a,
     for (int n = 0; n != NT; ++n) {
         // the four lanes of a column hold sums over different keys
         l[n] = column_sum(l[n]);
+        l[n] = sum_of(a, wk, row[n].token < 0 ? -1 : row[n].limit, m[n], l[n]);
         if (row[n].token < 0) continue;
-        l[n] = sum_of(a, wk, row[n].limit, m[n], l[n]);
         // O^T: elements 16 t + 4 g + r of this lane's row
         if (wk.direct) {
             T* const dst = reinterpret_cast<T*>(a.out) + uint64_t(row[n].token) * a.out_stride +

@@ -205,3 +205,20 @@ def test_scores_of_minus_infinity(km, dtype, new, lens, shared):
     # no position at all: zeros
     b.table[:] = -1
     assert not attend(km, b, q, 0.1).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("new,page", [([1], 1), ([40, 1], 1), ([200, 90], 1), ([1] * 12, 8), ([90], 8)])
+def test_scores_of_minus_infinity_behind_missing_pages(km, dtype, new, page):
+    """Rows that end among the missing pages see nothing, those behind them only -inf."""
+    b = Paged(75, dtype, 2, 1, 64, page, new, [320] * len(new), 0)
+    q = queries(b)
+    q[..., 0] = 1
+    b.k[..., 0] = -np.inf
+    b.table[:, :280 // page] = -1
+    got = attend(km, b, q, 0.1)
+    for s in range(b.n_seqs):
+        at = np.arange(320 - new[s], 320)
+        rows = got[int(b.offsets[s]):int(b.offsets[s + 1])]
+        assert not rows[at < 280].any()
+        assert np.isnan(rows[at >= 280]).all()
