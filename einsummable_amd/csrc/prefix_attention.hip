@@ -19,10 +19,10 @@
 // Two kinds of workgroups.  attention_few_kernel, for decoding, bound by the bytes of K and V: tiles
 // of 16 rows; the four wavefronts of a workgroup take the steps of its keys in turn, straight from
 // global memory into registers (K and V are used once; in f16 a lane's four rows of V are transposed
-// there, v_perm_b32), and join their m, l and O at the end through LDS.  125 MB in 31 us, 4.0 TB/s.
+// there, v_perm_b32), and join their m, l and O at the end through LDS.  125 MB in 32 us, 3.9 TB/s.
 // attention_many_kernel, for the shared positions of a batch and for prompts, bound by the issue and
 // latency of its steps: each wavefront has 16 or 32 rows of its own and all of them go through the
-// same tiles of keys, staged in LDS.  30 GFLOP of prompts in 55 us, 0.55 PFLOP/s.
+// same tiles of keys, staged in LDS.  30 GFLOP of prompts in 69 us, 0.44 PFLOP/s.
 // attention_mixed_kernel has workgroups of both kinds.
 //
 // Work is cut over the keys: "prefix" workgroups take the rows of the whole batch against a cut
@@ -88,7 +88,9 @@ __device__ inline float scaled(float y, float by) { return finite(y) ? y * by : 
 // f16 products take a weight p as two numbers, the f16 next to p and the f16 next to what that
 // leaves: 22 bits of it, where one f16 has 11 and cost results of f16 half a step of their own.  So
 // that small weights have them too, weights are taken relative to 2^-WEIGHT_LIFT of their row's
-// reference: what is lost of each is below 2^-32 of the largest.
+// reference: what is lost of each is below 2^-32 of the largest.  It costs the kernel of many rows the
+// second product's matrix instructions once more and about sixty others in a step of 32 keys
+// (prompts 55 us with one f16, 69 us), the one of few rows, which waits for memory, nothing.
 constexpr int WEIGHT_LIFT = 7;
 
 __device__ inline void split_weights(float2_t p, half2_t& high, half2_t& low)
@@ -339,8 +341,8 @@ __device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int 
         each = units_per_piece<ROWS>(a, __builtin_amdgcn_readlane(wave_scan(tiles * per), 63));
         if (ROWS != FEW) {
             // The least size of which the batch has at most `shares` pieces, rests included, so
-            // that all run at once and there are fewer to join (prompts: 58 us where rests came
-            // second, 56 us).  More tiles than that: several rounds anyway.
+            // that all run at once and there are fewer to join (prompts: 87 us with the rests on
+            // top of `shares`, 69 us).  More tiles than that: several rounds anyway.
             int const count = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
             int       most = __builtin_amdgcn_readlane(wave_max(tiles > 0 ? per : 0), 63);
             if (count <= a.shares) {
@@ -482,8 +484,9 @@ __device__ inline bool piece(attention_dev_t const& a, deal_t& sh, int kvh, int 
 }
 
 // Keys and values that hardly any other workgroup reads, as f16 sequences of few rows are one tile:
-// not kept in the caches (32 heads of keys, 32 tokens: 49.2 us, 47.8 us with it).  In f32 every
-// tile has sixteen rows, and long ones read the same keys many times.
+// not kept in the caches (32 heads of keys, 32 tokens, a launch of their own: 49.2 us, 47.8 us with
+// it; in one launch with the shared positions 58 to 61 us either way).  In f32 every tile has sixteen
+// rows, and long ones read the same keys many times.
 template <typename V>
 __device__ inline V read_once(void const* p)
 {
@@ -1573,9 +1576,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attention_many_kern
 
 // The shared positions in tiles of many rows and the own ones in tiles of few, in one launch: the
 // former are bound by instructions, the latter by memory, and two workgroups of either kind fit a
-// compute unit (64 tokens over a prefix of 8192: 22 + 31 us one after the other, 48 us together; 32
-// tokens, 32 heads of keys: 12 + 48 us, 59 us).  The former come first; in turn with the latter
-// they took 56 us.
+// compute unit (64 tokens over a prefix of 8192: 26 + 32 us one after the other, 51 us together; 32
+// tokens, 32 heads of keys: 13 + 50 us, 61 us).  The former come first; in turn with the latter
+// 64 tokens took 56 us.
 template <int D, int NT, bool PAD>
 __global__ __launch_bounds__(THREADS, 2) void attention_mixed_kernel(attention_dev_t a)
 {
@@ -1594,8 +1597,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mixed_kernel(attention_d
 
 // The references and sums of a row's cuts decide their weights, then the cuts' O are added in a
 // fixed order: TEAMS teams of sixteen lanes per row take them in turn: four teams where many cuts are
-// to be joined (2048 rows of 17: 7.8 us, 8.8 us with one), one where many rows are (26784 rows of two:
-// 10.1 us, 20.8 us with four).  Bound by the partial results' bytes, 17 and 41 MB.
+// to be joined (2048 rows of 17: 8.4 us, 10.2 us with one), one where many rows are (26784 rows of
+// two: 10.6 us, 23.1 us with four).  Bound by the partial results' bytes, 17 and 41 MB.
 template <typename T, int D, int TEAMS>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(attention_dev_t a)
 {
@@ -1836,12 +1839,13 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
     if (shared > 0) {
         p.prefix_rows = tile_rows(c, rows);
         uint64_t const tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
-        // workgroups of few rows run four to a compute unit, and those of many are slowed by a
-        // second one (64 tokens: 22.8 us with 256, 27.4 with 384, 24.6 and 3 us more to join with 512)
+        // Workgroups of few rows run four to a compute unit, and those of many are slowed by a
+        // second one (64 tokens, with the own positions: 50.5 us with 256, 56.0 with 384, 66.7 and
+        // 3 us more to join with 512).  Measured at head_dim 128; at 256 two and one fit.
         uint64_t const slots = p.prefix_rows == FEW ? 1024 : 256;
         uint64_t const want = (slots + tiles * kv - 1) / (tiles * kv);
         // no cuts below 256 positions; below 128 for a single tile of few rows, where the time is a
-        // wavefront's steps one after the other (1 token, 512 shared: 6.4 us, 7.6 us in cuts of
+        // wavefront's steps one after the other (1 token, 512 shared: 7.2 us, 8.6 us in cuts of
         // 256; f32, 15 tiles, 777 shared: no faster, and the join 1 us slower)
         uint64_t const cut = p.prefix_rows == FEW && tiles == 1 ? 128 : 256;
         uint64_t const most = (shared + cut - 1) / cut;
@@ -1860,7 +1864,7 @@ attention_plan_t plan_attention(es_km_kv_cache_t const& c, int n_seqs, int n_tok
         tiles = std::min(tiles, seqs + (rows - seqs * group) / (p.own_rows - group + 1));
     }
     // as many as run at once, two or four to a compute unit (64 tokens in one launch with the prefix:
-    // 49 us with 1024, 48 us with 512)
+    // 55.7 us with 1024, 50.5 us with 512; head_dim 128, at 256 one or two fit)
     bool const     two = p.own_rows != FEW || mixed(c.dtype == ES_KM_F16, c.head_dim, p.prefix_splits,
                                                 p.prefix_rows, p.own_rows);
     uint64_t const aim = two ? 512 : 1024;
