@@ -257,9 +257,10 @@ int es_km_kv_append(es_km_t* km, const es_km_kv_cache_t* cache, const es_km_kv_b
  * position gets zeros; one that sees a NaN score, or no other score than -inf, gets NaN, as the
  * formula does.  What masked positions hold, infinities and NaN included, has no
  * influence; neither have cache entries beyond lens.  Infinities and NaN in values that a token
- * sees reach its result whatever their weight, which is positive (and cost a second pass).
- * Scores, weights, sums and results are fp32; in f16 the matrix unit gets each weight as two f16
- * parts, 22 bits of it, and what lies below 2^-32 of the largest weight is lost.
+ * sees reach its result whatever their weight, one of zero (a score of -inf) included; they cost a
+ * second pass.
+ * Scores, weights and sums are fp32, results are rounded once; in f16 the matrix unit gets each
+ * weight as two f16 parts, 22 bits of it, and what lies below 2^-32 of the largest weight is lost.
  * Batches of more tokens times heads than a launch holds (some 2^24 to 2^26) are refused.
  * q and out: n_heads heads per token, q_stride / out_stride elements from token to token, on
  * 16-byte boundaries; out may not overlap q or the cache.
